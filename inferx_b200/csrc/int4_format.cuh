@@ -1,0 +1,62 @@
+// Weights held in four bits: how a matrix is laid out, and how codes become numbers.
+//
+// A row is cut along K into groups of 32, 64 or 128 entries; entry = scale * (code - zero) with a
+// code and a zero point in 0..15 and a bfloat16 scale per row and group.
+//
+// Codes.  [matrix][strip of 16 rows][tile of 64 k][lane 0..31][word 0..3], K padded to a multiple of
+// 128: 512 bytes a tile, a strip's tiles one behind the other.  Lane 4 g + t holds rows g and g + 8
+// for the k of two runs of eight, 8 t .. 8 t + 7 and 32 + 8 t .. 32 + 8 t + 7; word 2 h + j has the
+// entries 4 j .. 4 j + 3 of run h.  Nibbles i and i + 4 of a word are a pair of neighbouring k:
+// i = 0, 1: the first pair of rows g and g + 8; i = 2, 3: the second.  So one 16-byte load of a lane is
+// the A side of four mma.m16n8k16 (k in an order that the activations' 16-byte loads follow too), and
+// the four lanes of a row hold 16-byte pieces that lie beside each other in a K-major operand tile.
+//
+// Parameters.  [matrix][strip][chunk of 128 k][row 0..15][group of the chunk]: one word, the scale in
+// the low half, 128 + zero as bfloat16 in the high half.  (The zero point as a nibble would be 1.5 of
+// 67 bytes a group less; the word needs no arithmetic before its use.)
+//
+// A code c becomes the bfloat16 128 + c by setting its bits below 0x4300, and 128 + c - (128 + zero)
+// is exact: products of activations with codes are formed from whole numbers of -15..15, summed in
+// fp32 over a group, and the group's scale multiplies the sum in fp32.  Padding codes equal their
+// group's zero point, padding rows and groups have scale 0.
+#pragma once
+#include "common.cuh"
+
+#define I4_STRIP 16                    // rows of a strip
+#define I4_TILE_WORDS 128              // 16 rows x 64 k
+#define I4_CHUNK_K 128                 // k of a chunk
+#define I4_CHUNK_WORDS 256             // a strip's codes of a chunk
+
+__host__ __device__ static inline long long i4_strips(long long rows) {
+  return (rows + I4_STRIP - 1) / I4_STRIP;
+}
+__host__ __device__ static inline long long i4_chunks(long long k) {
+  return (k + I4_CHUNK_K - 1) / I4_CHUNK_K;
+}
+
+__device__ __forceinline__ float i4_scale(unsigned param) { return __uint_as_float(param << 16); }
+// 128 + zero in both halves
+__device__ __forceinline__ unsigned i4_sub(unsigned param) { return __byte_perm(param, 0, 0x3232); }
+
+// Nibbles i and i + 4 of a word, less the zero point: two neighbouring k.
+__device__ __forceinline__ unsigned i4_pair(unsigned word, int i, unsigned sub) {
+  unsigned q = ((word >> (4 * i)) & 0x000f000fu) | 0x43004300u;
+  const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&q),
+                                   *reinterpret_cast<const __nv_bfloat162*>(&sub));
+  return *reinterpret_cast<const unsigned*>(&d);
+}
+
+// An fp32 number as three bfloat16 terms by cutting off: 8 + 8 + 8 bits, nothing is left over (down
+// to 2^-133, the last bit that bfloat16 has).  An infinity is its first term alone.
+__device__ __forceinline__ void i4_terms2(float a, float b, unsigned& t1, unsigned& t2,
+                                          unsigned& t3) {
+  const unsigned a1 = __float_as_uint(a) & 0xffff0000u, b1 = __float_as_uint(b) & 0xffff0000u;
+  t1 = __byte_perm(a1, b1, 0x7632);
+  a = fabsf(a) == INFINITY ? 0.f : a - __uint_as_float(a1);
+  b = fabsf(b) == INFINITY ? 0.f : b - __uint_as_float(b1);
+  const unsigned a2 = __float_as_uint(a) & 0xffff0000u, b2 = __float_as_uint(b) & 0xffff0000u;
+  t2 = __byte_perm(a2, b2, 0x7632);
+  a -= __uint_as_float(a2);
+  b -= __uint_as_float(b2);
+  t3 = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
+}

@@ -1,0 +1,363 @@
+// Making, laying out and reading back matrices of four-bit codes (int4_format.cuh).
+//
+// Quantising a group: lo = min(0, least entry), hi = max(0, greatest), scale = (hi - lo) / 15 rounded
+// once to bfloat16, zero = rint(-lo / scale), code = rint(entry / scale) + zero, both kept in 0..15.
+// A group of zeros (or so small that its scale is 0) has scale, zero point and codes 0; a group that
+// holds an infinity or a NaN has scale NaN, so that products say so.
+//
+// One warp takes 16 rows by 128 k: a lane holds the 64 entries whose codes it packs, least and greatest
+// entries are joined over the four lanes of a row by shuffles, nothing passes through shared memory, and
+// each entry is read once.  Bound by the bytes read and written.
+#include "int4_format.cuh"
+
+#define I4_WARPS 8
+
+// The nearest whole number to v / s (ties to even) for |v| <= 16 s.  v of 24 bits and s of 8: the
+// quotient can round onto a half, the remainder cannot.
+__device__ __forceinline__ float i4_rint_ratio(float v, float s) {
+  float q = rintf(__fdiv_rn(v, s));
+  const float left = fmaf(-q, s, v), half = 0.5f * s;
+  if (left > half) q += 1.f;
+  if (left < -half) q -= 1.f;
+  return q;
+}
+
+// (hi - lo) / 15 in 64 bits, cut to 32 with the last bit set where something was cut off, then
+// rounded to bfloat16: one rounding in all.
+__device__ __forceinline__ bf16 i4_group_scale(float lo, float hi) {
+  const double q = ((double)hi - (double)lo) / 15.0;
+  unsigned u = __float_as_uint(__double2float_rz(q));
+  if ((double)__uint_as_float(u) != q) u |= 1u;
+  return __float2bfloat16_rn(__uint_as_float(u));
+}
+
+__device__ __forceinline__ unsigned i4_param(bf16 scale, int zero) {
+  return (unsigned)__bfloat16_as_ushort(scale) | (0x43000000u + ((unsigned)zero << 16));
+}
+
+// Where a warp works: matrix, strip, chunk; false behind the last.
+struct I4Place {
+  long long m;
+  int strip, chunk;
+};
+__device__ __forceinline__ bool i4_place(I4Place& p, long long matrices, int strips, int chunks) {
+  const long long w = (long long)blockIdx.x * I4_WARPS + (threadIdx.x >> 5);
+  if (w >= matrices * strips * chunks) return false;
+  p.chunk = (int)(w % chunks);
+  const long long s = w / chunks;
+  p.strip = (int)(s % strips);
+  p.m = s / strips;
+  return true;
+}
+
+// The 32 entries of a row that a lane of `t` holds of a chunk, from `src` (the row, or null: zeros).
+template <typename T>
+__device__ __forceinline__ void i4_row_entries(const T* src, int k0, int K, int t, bool vec,
+                                               float* v) {
+#pragma unroll
+  for (int b = 0; b < 4; ++b) {                    // blocks of 32 k
+    const int k = k0 + b * 32 + t * 8;
+    if (vec && src && k < K) {                     // K is a multiple of 8
+      if (sizeof(T) == 2) {
+        const uint4 r = *reinterpret_cast<const uint4*>(src + k);
+        const unsigned u[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          v[b * 8 + 2 * i] = __uint_as_float(u[i] << 16);
+          v[b * 8 + 2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float4 r = *reinterpret_cast<const float4*>(src + k + 4 * i);
+          v[b * 8 + 4 * i] = r.x;
+          v[b * 8 + 4 * i + 1] = r.y;
+          v[b * 8 + 4 * i + 2] = r.z;
+          v[b * 8 + 4 * i + 3] = r.w;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        v[b * 8 + i] = (src && k + i < K) ? to_f32<T>(src[k + i]) : 0.f;
+    }
+  }
+}
+
+// codes of rows g and g + 8 (32 each, in the order of i4_row_entries) to the lane's words
+__device__ __forceinline__ void i4_store_words(unsigned* dst, int lane, const unsigned char* ca,
+                                               const unsigned char* cb) {
+#pragma unroll
+  for (int tile = 0; tile < 2; ++tile) {
+    unsigned w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {                  // word 2 h + j
+      const int at = tile * 16 + (i >> 1) * 8 + (i & 1) * 4;
+      w[i] = (unsigned)ca[at] | ((unsigned)ca[at + 1] << 16) | ((unsigned)cb[at] << 4) |
+             ((unsigned)cb[at + 1] << 20) | ((unsigned)ca[at + 2] << 8) |
+             ((unsigned)ca[at + 3] << 24) | ((unsigned)cb[at + 2] << 12) |
+             ((unsigned)cb[at + 3] << 28);
+    }
+    *reinterpret_cast<uint4*>(dst + tile * I4_TILE_WORDS + lane * 4) =
+        make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+template <typename T, int GROUP>
+__global__ void __launch_bounds__(I4_WARPS * 32)
+i4_quantize_kernel(const T* __restrict__ w, unsigned* __restrict__ codes,
+                   unsigned* __restrict__ params, long long matrices, int rows, int K, int strips,
+                   int chunks, int vec) {
+  constexpr int PER = GROUP / 32, NG = 4 / PER;    // blocks of 32 a group, groups a chunk
+  I4Place p;
+  if (!i4_place(p, matrices, strips, chunks)) return;
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int k0 = p.chunk * I4_CHUNK_K;
+  const size_t block = ((size_t)p.m * strips + p.strip) * chunks + p.chunk;
+  unsigned char code[2][32];
+#pragma unroll
+  for (int side = 0; side < 2; ++side) {
+    const int row = p.strip * I4_STRIP + g + side * 8;
+    const T* src = row < rows ? w + ((size_t)p.m * rows + row) * K : nullptr;
+    float v[32];
+    i4_row_entries<T>(src, k0, K, t, vec != 0, v);
+#pragma unroll
+    for (int n = 0; n < NG; ++n) {
+      float lo = 0.f, hi = 0.f;
+      bool bad = false;
+#pragma unroll
+      for (int i = 0; i < PER * 8; ++i) {
+        const float e = v[n * PER * 8 + i];
+        lo = fminf(lo, e);
+        hi = fmaxf(hi, e);
+        bad |= !(fabsf(e) < INFINITY);
+      }
+#pragma unroll
+      for (int o = 1; o < 4; o <<= 1) {
+        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+        bad |= __shfl_xor_sync(0xffffffffu, (int)bad, o) != 0;
+      }
+      bf16 scale = bad ? __ushort_as_bfloat16(0x7fc0) : i4_group_scale(lo, hi);
+      const float s = __bfloat162float(scale);
+      const bool some = s > 0.f;                   // false for 0 and for NaN
+      const float zero = some ? fminf(fmaxf(i4_rint_ratio(-lo, s), 0.f), 15.f) : 0.f;
+#pragma unroll
+      for (int i = 0; i < PER * 8; ++i) {
+        const int at = n * PER * 8 + i;
+        const float c = fminf(fmaxf(i4_rint_ratio(v[at], s) + zero, 0.f), 15.f);
+        code[side][at] = some ? (unsigned char)(int)c : 0;
+      }
+      if (t == 0) params[(block * I4_STRIP + g + side * 8) * NG + n] = i4_param(scale, (int)zero);
+    }
+  }
+  i4_store_words(codes + block * I4_CHUNK_WORDS, lane, code[0], code[1]);
+}
+
+// Codes, scales and zero points of a caller's own into the layout.
+template <int GROUP>
+__global__ void __launch_bounds__(I4_WARPS * 32)
+i4_pack_kernel(const unsigned char* __restrict__ in, const bf16* __restrict__ scales,
+               const unsigned char* __restrict__ zeros, unsigned* __restrict__ codes,
+               unsigned* __restrict__ params, long long matrices, int rows, int K, int strips,
+               int chunks, int vec) {
+  constexpr int PER = GROUP / 32, NG = 4 / PER;
+  I4Place p;
+  if (!i4_place(p, matrices, strips, chunks)) return;
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int k0 = p.chunk * I4_CHUNK_K, groups = (K + GROUP - 1) / GROUP;
+  const size_t block = ((size_t)p.m * strips + p.strip) * chunks + p.chunk;
+  unsigned char code[2][32];
+#pragma unroll
+  for (int side = 0; side < 2; ++side) {
+    const int row = p.strip * I4_STRIP + g + side * 8;
+    const size_t r = (size_t)p.m * rows + row;
+#pragma unroll
+    for (int n = 0; n < NG; ++n) {
+      const int group = p.chunk * NG + n;
+      const bool there = row < rows && group < groups;
+      const bf16 scale = there ? scales[r * groups + group] : __ushort_as_bfloat16(0);
+      const int zero = there ? zeros[r * groups + group] & 15 : 0;
+#pragma unroll
+      for (int b = 0; b < PER; ++b) {
+        const int at = (n * PER + b) * 8, k = k0 + (n * PER + b) * 32 + t * 8;
+        if (vec && there && k < K) {               // K is a multiple of 8
+          const uint2 q = *reinterpret_cast<const uint2*>(in + r * K + k);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            code[side][at + i] = (q.x >> (8 * i)) & 15;
+            code[side][at + 4 + i] = (q.y >> (8 * i)) & 15;
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            code[side][at + i] = there && k + i < K ? in[r * K + k + i] & 15 : zero;
+        }
+      }
+      if (t == 0) params[(block * I4_STRIP + g + side * 8) * NG + n] = i4_param(scale, zero);
+    }
+  }
+  i4_store_words(codes + block * I4_CHUNK_WORDS, lane, code[0], code[1]);
+}
+
+// The layout back to codes, scales and zero points.
+template <int GROUP>
+__global__ void __launch_bounds__(I4_WARPS * 32)
+i4_unpack_kernel(const unsigned* __restrict__ codes, const unsigned* __restrict__ params,
+                 unsigned char* __restrict__ out, bf16* __restrict__ scales,
+                 unsigned char* __restrict__ zeros, long long matrices, int rows, int K, int strips,
+                 int chunks, int vec) {
+  constexpr int NG = 128 / GROUP;
+  I4Place p;
+  if (!i4_place(p, matrices, strips, chunks)) return;
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int k0 = p.chunk * I4_CHUNK_K, groups = (K + GROUP - 1) / GROUP;
+  const size_t block = ((size_t)p.m * strips + p.strip) * chunks + p.chunk;
+  uint4 w[2];
+#pragma unroll
+  for (int tile = 0; tile < 2; ++tile)
+    w[tile] = *reinterpret_cast<const uint4*>(codes + block * I4_CHUNK_WORDS +
+                                              tile * I4_TILE_WORDS + lane * 4);
+#pragma unroll
+  for (int side = 0; side < 2; ++side) {
+    const int row = p.strip * I4_STRIP + g + side * 8;
+    if (row >= rows) continue;
+    const size_t r = (size_t)p.m * rows + row;
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      const int k = k0 + b * 32 + t * 8;
+      const uint4 q = w[b >> 1];
+      const unsigned lo = (b & 1) ? q.z : q.x, hi = (b & 1) ? q.w : q.y;
+      unsigned o[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {                // four codes of a row out of a word
+        const unsigned u = (j ? hi : lo) >> (4 * side);
+        o[j] = (u & 15) | ((u >> 16 & 15) << 8) | ((u >> 8 & 15) << 16) | ((u >> 24 & 15) << 24);
+      }
+      if (vec && k < K) {
+        *reinterpret_cast<uint2*>(out + r * K + k) = make_uint2(o[0], o[1]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (k + i < K) out[r * K + k + i] = (unsigned char)(o[i >> 2] >> (8 * (i & 3)));
+      }
+    }
+    for (int n = t; n < NG; n += 4) {
+      const int group = p.chunk * NG + n;
+      if (group >= groups) continue;
+      const unsigned param = params[(block * I4_STRIP + g + side * 8) * NG + n];
+      scales[r * groups + group] = __ushort_as_bfloat16((unsigned short)param);
+      zeros[r * groups + group] = (unsigned char)((param >> 16) - 0x4300u);
+    }
+  }
+}
+
+static int i4_grid(long long matrices, int rows, int K, int& strips, int& chunks, unsigned& grid) {
+  if (matrices <= 0 || rows <= 0 || K <= 0) return IX_ERR_SIZE;
+  strips = (int)i4_strips(rows);
+  chunks = (int)i4_chunks(K);
+  const long long blocks = (matrices * strips * chunks + I4_WARPS - 1) / I4_WARPS;
+  if (blocks > 0x7fffffffLL) return IX_ERR_SIZE;
+  grid = (unsigned)blocks;
+  return IX_OK;
+}
+
+#define I4_GROUPS(G, ...)                                                      \
+  do {                                                                         \
+    if (group == 128) { constexpr int G = 128; __VA_ARGS__; }                  \
+    else if (group == 64) { constexpr int G = 64; __VA_ARGS__; }               \
+    else if (group == 32) { constexpr int G = 32; __VA_ARGS__; }               \
+    else return IX_ERR_UNSUPPORTED;                                            \
+  } while (0)
+
+// w: [matrices, rows, K] fp32 or bf16.  codes: [matrices, strips, chunks, 256] words; params:
+// [matrices, strips, chunks, 16, 128 / group] words.
+IX_API int ix_int4_quantize(const void* w, int dtype, void* codes, void* params,
+                            long long matrices, int rows, int K, int group, cudaStream_t stream) {
+  int strips, chunks;
+  unsigned grid;
+  const int rc = i4_grid(matrices, rows, K, strips, chunks, grid);
+  if (rc != IX_OK) return rc;
+  const int vec = K % 8 == 0 && ((uintptr_t)w & 15) == 0;
+  IX_DISPATCH_DTYPE(dtype, T, {
+    I4_GROUPS(G, i4_quantize_kernel<T, G><<<grid, I4_WARPS * 32, 0, stream>>>(
+                     (const T*)w, (unsigned*)codes, (unsigned*)params, matrices, rows, K, strips,
+                     chunks, vec));
+  });
+  return ix_launch_status();
+}
+
+// in: [matrices, rows, K] bytes; scales bf16 and zeros bytes: [matrices, rows, ceil(K / group)].
+IX_API int ix_int4_pack(const void* in, const void* scales, const void* zeros, void* codes,
+                        void* params, long long matrices, int rows, int K, int group,
+                        cudaStream_t stream) {
+  int strips, chunks;
+  unsigned grid;
+  const int rc = i4_grid(matrices, rows, K, strips, chunks, grid);
+  if (rc != IX_OK) return rc;
+  const int vec = K % 8 == 0 && ((uintptr_t)in & 7) == 0;
+  I4_GROUPS(G, i4_pack_kernel<G><<<grid, I4_WARPS * 32, 0, stream>>>(
+                   (const unsigned char*)in, (const bf16*)scales, (const unsigned char*)zeros,
+                   (unsigned*)codes, (unsigned*)params, matrices, rows, K, strips, chunks, vec));
+  return ix_launch_status();
+}
+
+IX_API int ix_int4_unpack(const void* codes, const void* params, void* out, void* scales,
+                          void* zeros, long long matrices, int rows, int K, int group,
+                          cudaStream_t stream) {
+  int strips, chunks;
+  unsigned grid;
+  const int rc = i4_grid(matrices, rows, K, strips, chunks, grid);
+  if (rc != IX_OK) return rc;
+  const int vec = K % 8 == 0 && ((uintptr_t)out & 7) == 0;
+  I4_GROUPS(G, i4_unpack_kernel<G><<<grid, I4_WARPS * 32, 0, stream>>>(
+                   (const unsigned*)codes, (const unsigned*)params, (unsigned char*)out,
+                   (bf16*)scales, (unsigned char*)zeros, matrices, rows, K, strips, chunks, vec));
+  return ix_launch_status();
+}
+
+// Activation rows as the products want them: gathered where `rows` names them, with zeros from K up to
+// Kp, in their own type (TERMS 1) or as three planes of bfloat16 terms (fp32, TERMS 3).
+template <typename T, int TERMS>
+__global__ void __launch_bounds__(128)
+i4_rows_kernel(const T* __restrict__ x, const int* __restrict__ rows, void* __restrict__ out, int R,
+               int K, int Kp) {
+  IX_PDL_WAIT();
+  const size_t r = blockIdx.x, src = rows ? (size_t)rows[r] : r;
+  for (int k = 2 * threadIdx.x; k < Kp; k += 256) {    // Kp is even
+    const float a = k < K ? to_f32<T>(x[src * K + k]) : 0.f;
+    const float b = k + 1 < K ? to_f32<T>(x[src * K + k + 1]) : 0.f;
+    if (TERMS == 3) {
+      unsigned t1, t2, t3;
+      i4_terms2(a, b, t1, t2, t3);
+      unsigned* o = (unsigned*)out + (r * Kp + k) / 2;
+      const size_t plane = (size_t)R * Kp / 2;
+      o[0] = t1;
+      o[plane] = t2;
+      o[2 * plane] = t3;
+    } else {
+      T* o = (T*)out + r * Kp + k;
+      o[0] = from_f32<T>(a);
+      o[1] = from_f32<T>(b);
+    }
+  }
+}
+
+IX_API int ix_int4_rows(const void* x, int dtype, const int* rows, void* out, int R, int K, int Kp,
+                        int terms, cudaStream_t stream) {
+  if (R <= 0) return IX_OK;
+  if (K <= 0 || Kp < K || Kp % 8) return IX_ERR_SIZE;
+  if ((uintptr_t)out & 15) return IX_ERR_ALIGN;
+  if (terms == 3 && dtype == IX_F32)
+    ix_launch(i4_rows_kernel<float, 3>, dim3(R), dim3(128), 0, stream, (const float*)x, rows, out, R,
+              K, Kp);
+  else if (terms == 1 && dtype == IX_F32)
+    ix_launch(i4_rows_kernel<float, 1>, dim3(R), dim3(128), 0, stream, (const float*)x, rows, out, R,
+              K, Kp);
+  else if (terms == 1 && dtype == IX_BF16)
+    ix_launch(i4_rows_kernel<bf16, 1>, dim3(R), dim3(128), 0, stream, (const bf16*)x, rows, out, R,
+              K, Kp);
+  else
+    return IX_ERR_UNSUPPORTED;
+  return ix_launch_status();
+}

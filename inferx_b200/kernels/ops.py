@@ -271,6 +271,8 @@ def activate(x: torch.Tensor, activation: str, out: Optional[torch.Tensor] = Non
 def linear_act(x: torch.Tensor, w: torch.Tensor, activation: str):
     """act(x[M,K] . w[N,K]^T): in the product's epilogue where this library's kernels run it,
     else in place over the library's result."""
+    if isinstance(w, Int4Weight):
+        return _int4_product("linear_act", x, w, 1, activation=activation)
     _chk("x", x)
     _chk("w", w, x.dtype)
     M = x.shape[0]
@@ -286,7 +288,10 @@ def linear_act(x: torch.Tensor, w: torch.Tensor, activation: str):
 
 
 def linear(x: torch.Tensor, w: torch.Tensor, out_dtype: Optional[torch.dtype] = None):
-    """x[M,K] . w[N,K]^T.  bfloat16: cuBLAS, fp32 accumulation.  float32: own kernels."""
+    """x[M,K] . w[N,K]^T.  bfloat16: cuBLAS, fp32 accumulation.  float32: own kernels; own
+    kernels too where ``w`` is an ``Int4Weight``."""
+    if isinstance(w, Int4Weight):
+        return _int4_product("linear", x, w, 1, out_dtype=out_dtype)
     _chk("x", x)
     _chk("w", w)
     if x.dtype != w.dtype:
@@ -443,6 +448,8 @@ def qkv_project_applies(x: torch.Tensor, w: torch.Tensor, heads: int, kv_heads: 
                         head_dim: int, rotary_dim: int) -> bool:
     """Whether ``qkv_project_rope_append`` takes this step: bfloat16, a few tokens, a full
     rotation or none."""
+    if isinstance(w, Int4Weight):
+        return False
     return bool(USE_FUSED_QKV and x.is_cuda and x.dtype == torch.bfloat16
                 and w.dtype == torch.bfloat16 and x.is_contiguous()
                 and _lib().ix_qkv_project_rope_applies(x.shape[0], x.shape[1], heads, kv_heads,
@@ -1424,6 +1431,9 @@ def grouped_gate_up_swiglu(x: torch.Tensor, rows: torch.Tensor, offsets: torch.T
         _chk("row_scale", row_scale, torch.float32)
         if row_scale.numel() != A:
             raise KernelError("grouped_gate_up_swiglu: one factor per grouped row")
+    if isinstance(w_gate_up, Int4Weight):
+        return _int4_grouped("grouped_gate_up_swiglu", x, rows, offsets, w_gate_up, 2,
+                             row_scale=row_scale)
     per = A / w_gate_up.shape[0]
     if _stream_grouped_applies(x, w_gate_up, A):
         return gemm_stream_grouped(x, w_gate_up, rows, offsets, True, A,
@@ -1442,6 +1452,8 @@ def grouped_up(x: torch.Tensor, rows: torch.Tensor, offsets: torch.Tensor, w_up:
                activation: str):
     """act[r] = activation(x[rows[r]] . Wu[e]^T), e from offsets: experts without a gate,
     ``w_up`` [E, I, H]."""
+    if isinstance(w_up, Int4Weight):
+        return _int4_grouped("grouped_up", x, rows, offsets, w_up, 1, activation=activation)
     A = rows.numel()
     per = A / w_up.shape[0]
     if _stream_grouped_applies(x, w_up, A):
@@ -1460,6 +1472,9 @@ def grouped_down(act: torch.Tensor, offsets: torch.Tensor, w_down: torch.Tensor,
     """y[r] = act[r] . Wd[e]^T with ``w_down`` [E, H, I].  ``offsets_settled``: see
     ``gemm_small_m`` (true when this follows ``grouped_gate_up_swiglu`` on the same
     offsets, as in a mixture layer)."""
+    if isinstance(w_down, Int4Weight):
+        return _int4_grouped("grouped_down", act, None, offsets, w_down, 1,
+                             offsets_settled=offsets_settled)
     A = act.shape[0]
     per = A / w_down.shape[0]
     if _stream_grouped_applies(act, w_down, A):
@@ -1475,12 +1490,220 @@ def grouped_down(act: torch.Tensor, offsets: torch.Tensor, w_down: torch.Tensor,
 
 def gate_up_swiglu(x: torch.Tensor, w_gate_up: torch.Tensor):
     """Dense SwiGLU front half: silu(x . Wg^T) * (x . Wu^T) with ``w_gate_up`` [2I, H]."""
+    if isinstance(w_gate_up, Int4Weight):
+        return _int4_product("gate_up_swiglu", x, w_gate_up, 2)
     _chk("x", x)
     _chk("w_gate_up", w_gate_up, x.dtype)
     M = x.shape[0]
     if M <= SMALL_M_DENSE_ROWS and _streams_weights(x, w_gate_up):
         return gemm_small_m(x, w_gate_up.unsqueeze(0), None, None, True, M, rows_per_pass=M)
     return silu_mul(linear(x, w_gate_up))
+
+
+# ---------------------------------------------------------------------------
+# Weights held in four bits (csrc/int4_format.cuh)
+# ---------------------------------------------------------------------------
+INT4_GROUPS = (32, 64, 128)
+INT4_LAYOUT_ROWS, INT4_LAYOUT_K = 16, 128     # a strip of rows, a chunk of k
+
+
+class Int4Weight:
+    """A matrix ``[rows, K]``, or one per expert ``[E, rows, K]``, in four bits: per row and
+    group of ``group_size`` entries along K a bfloat16 scale and a zero point in 0..15, per entry
+    a code in 0..15 that stands for ``scale * (code - zero)``.  Made by ``quantize_int4`` or
+    ``pack_int4``; ``linear`` and the gated and grouped products take it where they take a
+    matrix.  ``halves`` is 2 where the rows are a gate matrix and then an up matrix of the same
+    size, which the gated products want, and 1 otherwise.  ``codes`` and ``params`` are int32
+    tensors in the kernels' own layout."""
+
+    __slots__ = ("shape", "halves", "group_size", "codes", "params")
+
+    def __init__(self, shape, halves: int, group_size: int, codes: torch.Tensor,
+                 params: torch.Tensor):
+        self.shape = torch.Size(shape)
+        self.halves, self.group_size = halves, group_size
+        self.codes, self.params = codes, params
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    @property
+    def experts(self) -> int:
+        return self.shape[0] if len(self.shape) == 3 else 1
+
+    @property
+    def cols(self) -> int:
+        """Output columns of a product: the rows of one half."""
+        return self.shape[-2] // self.halves
+
+    @property
+    def nbytes(self) -> int:
+        return self.codes.nbytes + self.params.nbytes
+
+    def numel(self) -> int:
+        return self.shape.numel()
+
+    def __repr__(self):
+        return (f"Int4Weight({list(self.shape)}, group_size={self.group_size}, "
+                f"halves={self.halves})")
+
+
+def _int4_empty(what: str, shape, group_size: int, halves: int, device) -> Int4Weight:
+    if len(shape) not in (2, 3) or 0 in shape:
+        raise KernelError(f"{what}: a matrix [rows, K] or [experts, rows, K] is wanted, "
+                          f"got {list(shape)}")
+    if group_size not in INT4_GROUPS:
+        raise KernelError(f"{what}: groups of {group_size} are not built ({INT4_GROUPS})")
+    if halves not in (1, 2) or shape[-2] % halves:
+        raise KernelError(f"{what}: {shape[-2]} rows in {halves} halves")
+    matrices = (shape[0] if len(shape) == 3 else 1) * halves
+    strips = -(-(shape[-2] // halves) // INT4_LAYOUT_ROWS)
+    chunks = -(-shape[-1] // INT4_LAYOUT_K)
+    codes = torch.empty((matrices, strips, chunks, 256), dtype=torch.int32, device=device)
+    params = torch.empty((matrices, strips, chunks, 16, 128 // group_size), dtype=torch.int32,
+                         device=device)
+    return Int4Weight(shape, halves, group_size, codes, params)
+
+
+def _on_current_device(what: str, *tensors):
+    """Kernels launch on the current device's stream: operands of another one are refused."""
+    now = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.device.index != now:
+            raise KernelError(f"{what}: an operand is on {t.device}, the current device is "
+                              f"cuda:{now}")
+
+
+def quantize_int4(w: torch.Tensor, group_size: int = 128, halves: int = 1) -> Int4Weight:
+    """``w`` [rows, K] or [E, rows, K] (bfloat16 or float32) in four bits.  Per row and group:
+    lo = min(0, least entry), hi = max(0, greatest), scale = (hi - lo) / 15 rounded once to
+    bfloat16, zero = rint(-lo / scale), code = rint(entry / scale) + zero, both kept in 0..15.
+    A group of zeros has scale 0; one that holds an infinity or a NaN has scale NaN."""
+    _chk("w", w)
+    code = _dtype_code(w)
+    _on_current_device("quantize_int4", w)
+    q = _int4_empty("quantize_int4", w.shape, group_size, halves, w.device)
+    _check(_lib().ix_int4_quantize(_ptr(w), code, _ptr(q.codes), _ptr(q.params),
+                                   ctypes.c_longlong(q.experts * halves), q.cols, w.shape[-1],
+                                   group_size, _stream()), "quantize_int4")
+    _count()
+    return q
+
+
+def pack_int4(codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor,
+              group_size: int = 128, halves: int = 1) -> Int4Weight:
+    """An ``Int4Weight`` from ``codes`` [.., rows, K] and ``zeros`` [.., rows, ceil(K /
+    group_size)] (uint8, 0..15) and ``scales`` (bfloat16, like ``zeros``).  Looks at the codes
+    on the host: for loading, not for a step."""
+    _chk("codes", codes, torch.uint8)
+    _chk("scales", scales, torch.bfloat16)
+    _chk("zeros", zeros, torch.uint8)
+    _on_current_device("pack_int4", codes, scales, zeros)
+    q = _int4_empty("pack_int4", codes.shape, group_size, halves, codes.device)
+    want = (*codes.shape[:-1], -(-codes.shape[-1] // group_size))
+    if tuple(scales.shape) != want or tuple(zeros.shape) != want:
+        raise KernelError(f"pack_int4: scales and zeros must be {list(want)}, got "
+                          f"{list(scales.shape)} and {list(zeros.shape)}")
+    if int(torch.maximum(codes.max(), zeros.max())) > 15:
+        raise KernelError("pack_int4: codes and zeros must lie in 0..15")
+    _check(_lib().ix_int4_pack(_ptr(codes), _ptr(scales), _ptr(zeros), _ptr(q.codes),
+                               _ptr(q.params), ctypes.c_longlong(q.experts * halves), q.cols,
+                               codes.shape[-1], group_size, _stream()), "pack_int4")
+    _count()
+    return q
+
+
+def unpack_int4(w: Int4Weight):
+    """(codes, scales, zeros) of an ``Int4Weight``, as ``pack_int4`` takes them."""
+    if not isinstance(w, Int4Weight):
+        raise KernelError(f"unpack_int4: expected an Int4Weight, got {type(w).__name__}")
+    _on_current_device("unpack_int4", w.codes)
+    groups = (*w.shape[:-1], -(-w.shape[-1] // w.group_size))
+    codes = torch.empty(w.shape, dtype=torch.uint8, device=w.device)
+    scales = torch.empty(groups, dtype=torch.bfloat16, device=w.device)
+    zeros = torch.empty(groups, dtype=torch.uint8, device=w.device)
+    _check(_lib().ix_int4_unpack(_ptr(w.codes), _ptr(w.params), _ptr(codes), _ptr(scales),
+                                 _ptr(zeros), ctypes.c_longlong(w.experts * w.halves), w.cols,
+                                 w.shape[-1], w.group_size, _stream()), "unpack_int4")
+    _count()
+    return codes, scales, zeros
+
+
+def _int4_operands(what: str, x: torch.Tensor, w: Int4Weight, halves: int, dims: int,
+                   *others) -> int:
+    """The checks that every product with an ``Int4Weight`` makes; the code of x's type."""
+    _chk("x", x)
+    code = _dtype_code(x)
+    _on_current_device(what, x, w.codes, *others)
+    if x.dim() != 2 or len(w.shape) != dims or x.shape[1] != w.shape[-1]:
+        raise KernelError(f"{what}: activations {list(x.shape)} against weights "
+                          f"{list(w.shape)}")
+    if w.halves != halves:
+        raise KernelError(f"{what}: weights of {w.halves} halves, {halves} wanted")
+    return code
+
+
+def _int4_rows(x: torch.Tensor, rows: Optional[torch.Tensor], terms: int) -> torch.Tensor:
+    """x (its listed rows) with columns up to a multiple of 8; three bfloat16 planes if asked."""
+    R = x.shape[0] if rows is None else rows.numel()
+    K = x.shape[1]
+    Kp = (K + 7) // 8 * 8
+    shape, dtype = ((3, R, Kp), torch.bfloat16) if terms == 3 else ((R, Kp), x.dtype)
+    out = torch.empty(shape, dtype=dtype, device=x.device)
+    _check(_lib().ix_int4_rows(_ptr(x), _dtype_code(x), _ptr(rows), _ptr(out), R, K, Kp, terms,
+                               _stream()), "int4_rows")
+    _count()
+    return out
+
+
+def _int4_stream(what, x, rows, offsets, w, num_rows, out_dtype, rows_per_pass, active=0,
+                 offsets_settled=False, row_scale=None, activation=None):
+    """Few rows: the codes stream past the activations (csrc/int4_stream.cu)."""
+    if x.shape[1] % 8 or x.data_ptr() % 16:
+        x, rows = _int4_rows(x, rows, 1), None
+        offsets_settled = False            # one launch more in front of this one
+    out = torch.empty((num_rows, w.cols), dtype=out_dtype, device=x.device)
+    _check(_lib().ix_int4_stream(
+        _ptr(x), _dtype_code(x), _ptr(rows), _ptr(offsets), _ptr(w.codes), _ptr(w.params),
+        _ptr(out), 1 if out_dtype == torch.float32 else 0, w.halves - 1,
+        0 if offsets is not None else num_rows, w.cols, x.shape[1], w.experts, w.group_size,
+        rows_per_pass, active, 1 if offsets_settled else 0, _ptr(row_scale),
+        _ACTIVATIONS[activation], _stream()), what)
+    _count()
+    return out
+
+
+def _int4_product(what: str, x: torch.Tensor, w: Int4Weight, halves: int,
+                  out_dtype: Optional[torch.dtype] = None, activation: Optional[str] = None):
+    """One matrix: x . w^T, gated where there are two halves."""
+    _int4_operands(what, x, w, halves, 2)
+    out_dtype = out_dtype or x.dtype
+    if out_dtype not in (torch.float32, x.dtype):
+        raise KernelError(f"{what}: results in {out_dtype} from activations in {x.dtype}")
+    M = x.shape[0]
+    if M == 0:
+        return torch.empty((0, w.cols), dtype=out_dtype, device=x.device)
+    return _int4_stream(what, x, None, None, w, M, out_dtype, M, activation=activation)
+
+
+def _int4_grouped(what: str, x: torch.Tensor, rows: Optional[torch.Tensor],
+                  offsets: torch.Tensor, w: Int4Weight, halves: int,
+                  offsets_settled: bool = False, row_scale: Optional[torch.Tensor] = None,
+                  activation: Optional[str] = None):
+    """One matrix per expert, ragged rows."""
+    _chk("rows", rows, torch.int32, optional=True)
+    _chk("offsets", offsets, torch.int32)
+    _int4_operands(what, x, w, halves, 3, rows, offsets, row_scale)
+    A = x.shape[0] if rows is None else rows.numel()
+    if offsets.numel() != w.experts + 1:
+        raise KernelError(f"{what}: offsets must have one entry per expert plus one")
+    if A == 0:
+        return torch.empty((0, w.cols), dtype=x.dtype, device=x.device)
+    per = A / w.experts
+    return _int4_stream(what, x, rows, offsets, w, A, x.dtype, 8 if per <= 2 else 16,
+                        active=min(w.experts, A), offsets_settled=offsets_settled,
+                        row_scale=row_scale, activation=activation)
 
 
 # ---------------------------------------------------------------------------

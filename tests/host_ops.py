@@ -43,6 +43,60 @@ def silu_mul(gu):
     return (g / (1.0 + torch.exp(-g)) * u).to(gu.dtype)
 
 
+class HostInt4:
+    """Codes, scales and zero points of a matrix in four bits, in the order of its entries."""
+
+    def __init__(self, codes, scales, zeros, group_size, halves):
+        self.codes, self.scales, self.zeros = codes, scales, zeros
+        self.group_size, self.halves, self.shape = group_size, halves, codes.shape
+
+    def numel(self):
+        return self.shape.numel()
+
+    @property
+    def nbytes(self):
+        return self.codes.numel() // 2 + self.scales.numel() * 4
+
+    def dense(self, dtype=torch.float32):
+        of = torch.arange(self.shape[-1], device=self.codes.device) // self.group_size
+        return ((self.codes.to(dtype) - self.zeros.to(dtype)[..., of])
+                * self.scales.to(dtype)[..., of])
+
+    # (the fp32 statements below see the matrix)
+    def to(self, dtype):
+        return self.dense(dtype)
+
+    def __getitem__(self, e):
+        return HostInt4(self.codes[e], self.scales[e], self.zeros[e], self.group_size, self.halves)
+
+
+def bf16_of(t):
+    """float64 >= 0 to bfloat16 in one rounding (to nearest, ties to even)."""
+    m, e = torch.frexp(t)
+    return torch.ldexp(torch.round(m * 256.0) / 256.0, e).to(torch.bfloat16)
+
+
+def quantize_int4(w, group_size=128, halves=1):
+    """Per row and group: lo = min(0, least), hi = max(0, greatest), scale = (hi - lo) / 15,
+    zero = rint(-lo / scale), code = rint(entry / scale) + zero; in 64 bits."""
+    K = w.shape[-1]
+    codes = torch.zeros(w.shape, dtype=torch.uint8, device=w.device)
+    scales, zeros = [], []
+    for k0 in range(0, K, group_size):
+        part = w[..., k0:k0 + group_size].double()
+        lo, hi = part.amin(-1).clamp(max=0.0), part.amax(-1).clamp(min=0.0)
+        bad = ~torch.isfinite(part).all(-1)
+        scale = bf16_of(torch.where(bad, 0.0, (hi - lo) / 15.0))
+        some = scale > 0
+        s = torch.where(some, scale.double(), 1.0)
+        zero = torch.where(some, torch.round(-lo / s).clamp(0, 15), 0.0)
+        code = (torch.round(part / s[..., None]) + zero[..., None]).clamp(0, 15)
+        codes[..., k0:k0 + group_size] = torch.where(some[..., None], code, 0.0).to(torch.uint8)
+        scales.append(torch.where(bad, torch.nan, scale.double()).to(torch.bfloat16))
+        zeros.append(zero.to(torch.uint8))
+    return HostInt4(codes, torch.stack(scales, -1), torch.stack(zeros, -1), group_size, halves)
+
+
 def linear(x, w, out_dtype=None):
     return (_f(x) @ _f(w).T).to(out_dtype or x.dtype)
 
