@@ -1341,6 +1341,7 @@ _STATUS_ROLES = {
     33: "widened_attention: a softmax warp",
     34: "widened_attention: shared memory not on a 1024-byte mark;",
     41: "gemm_fp32_tc: a splitting warp", 42: "gemm_fp32_tc: the MMA issuer",
+    51: "int4_tc: the copying warp", 52: "int4_tc: the MMA issuer", 53: "int4_tc: an unpacking warp",
 }
 
 
@@ -1674,6 +1675,30 @@ def _int4_stream(what, x, rows, offsets, w, num_rows, out_dtype, rows_per_pass, 
     return out
 
 
+# Up to this many rows of one matrix, or rows an expert on average, the codes stream past them;
+# beyond, the tcgen05 kernel.
+INT4_STREAM_ROWS = 32
+INT4_STREAM_ROWS_PER_GROUP = 2
+INT4_TC_MAX_EXPERTS = 1024
+
+
+def _int4_tc(what, x, rows, offsets, w, num_rows, out_dtype, row_scale=None, activation=None):
+    """Many rows, on the 5th-generation tensor cores (csrc/int4_tc.cu)."""
+    terms = 3 if x.dtype == torch.float32 else 1
+    if terms == 3 or x.shape[1] % 8 or x.data_ptr() % 16:
+        x = _int4_rows(x, rows, terms)
+    elif rows is not None:
+        x = gather_rows(x, rows)
+    out = torch.empty((num_rows, w.cols), dtype=out_dtype, device=x.device)
+    _check(_lib().ix_int4_tc(
+        _ptr(x), terms, _ptr(offsets), _ptr(w.codes), _ptr(w.params), _ptr(out),
+        1 if out_dtype == torch.float32 else 0, w.halves - 1, num_rows, w.cols, x.shape[-1],
+        w.experts, w.group_size, _ptr(row_scale), _ACTIVATIONS[activation],
+        _ptr(_tc_status(x.device)), _stream()), what)
+    _count()
+    return out
+
+
 def _int4_product(what: str, x: torch.Tensor, w: Int4Weight, halves: int,
                   out_dtype: Optional[torch.dtype] = None, activation: Optional[str] = None):
     """One matrix: x . w^T, gated where there are two halves."""
@@ -1684,6 +1709,8 @@ def _int4_product(what: str, x: torch.Tensor, w: Int4Weight, halves: int,
     M = x.shape[0]
     if M == 0:
         return torch.empty((0, w.cols), dtype=out_dtype, device=x.device)
+    if M > INT4_STREAM_ROWS:
+        return _int4_tc(what, x, None, None, w, M, out_dtype, activation=activation)
     return _int4_stream(what, x, None, None, w, M, out_dtype, M, activation=activation)
 
 
@@ -1701,6 +1728,9 @@ def _int4_grouped(what: str, x: torch.Tensor, rows: Optional[torch.Tensor],
     if A == 0:
         return torch.empty((0, w.cols), dtype=x.dtype, device=x.device)
     per = A / w.experts
+    if per > INT4_STREAM_ROWS_PER_GROUP and w.experts <= INT4_TC_MAX_EXPERTS:
+        return _int4_tc(what, x, rows, offsets, w, A, x.dtype, row_scale=row_scale,
+                        activation=activation)
     return _int4_stream(what, x, rows, offsets, w, A, x.dtype, 8 if per <= 2 else 16,
                         active=min(w.experts, A), offsets_settled=offsets_settled,
                         row_scale=row_scale, activation=activation)
