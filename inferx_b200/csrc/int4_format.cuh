@@ -3,17 +3,21 @@
 // A row is cut along K into groups of 32, 64 or 128 entries; entry = scale * (code - zero) with a
 // code and a zero point in 0..15 and a bfloat16 scale per row and group.
 //
-// Codes.  [matrix][strip of 16 rows][tile of 64 k][lane 0..31][word 0..3], K padded to a multiple of
-// 128: 512 bytes a tile, a strip's tiles one behind the other.  Lane 4 g + t holds rows g and g + 8
-// for the k of two runs of eight, 8 t .. 8 t + 7 and 32 + 8 t .. 32 + 8 t + 7; word 2 h + j has the
-// entries 4 j .. 4 j + 3 of run h.  Nibbles i and i + 4 of a word are a pair of neighbouring k:
-// i = 0, 1: the first pair of rows g and g + 8; i = 2, 3: the second.  So one 16-byte load of a lane is
-// the A side of four mma.m16n8k16 (k in an order that the activations' 16-byte loads follow too), and
-// the four lanes of a row hold 16-byte pieces that lie beside each other in a K-major operand tile.
+// Blocks.  [matrix][chunk of 128 k][strip of 16 rows], K padded to whole chunks and rows to whole
+// strips; a block is 256 words of codes and 16 x (128 / group) words of parameters behind them.  So the
+// strips that a tile of weight rows takes of a chunk are one piece of memory (one bulk copy), and a
+// strip's share of it is 1 KB and its parameters.
 //
-// Parameters.  [matrix][strip][chunk of 128 k][row 0..15][group of the chunk]: one word, the scale in
-// the low half, 128 + zero as bfloat16 in the high half.  (The zero point as a nibble would be 1.5 of
-// 67 bytes a group less; the word needs no arithmetic before its use.)
+// Codes.  [tile of 64 k][lane 0..31][word 0..3].  Lane 4 g + t holds rows g and g + 8 for the k of two
+// runs of eight, 8 t .. 8 t + 7 and 32 + 8 t .. 32 + 8 t + 7; word 2 h + j has the entries 4 j .. 4 j + 3
+// of run h.  Nibbles i and i + 4 of a word are a pair of neighbouring k: i = 0, 1: the first pair of
+// rows g and g + 8; i = 2, 3: the second.  So 16 bytes of a lane are the A side of four mma.m16n8k16
+// (k in an order that the activations' 16-byte loads follow too), and the four lanes of a row hold
+// 16-byte pieces that lie beside each other in a K-major operand tile.
+//
+// Parameters.  [row 0..15][group of the chunk]: one word, the scale in the low half, 128 + zero as
+// bfloat16 in the high half.  (The zero point as a nibble would be 1.5 of 67 bytes a group less; the
+// word needs no arithmetic before its use.)
 //
 // A code c becomes the bfloat16 128 + c by setting its bits below 0x4300, and 128 + c - (128 + zero)
 // is exact: products of activations with codes are formed from whole numbers of -15..15, summed in
@@ -25,7 +29,10 @@
 #define I4_STRIP 16                    // rows of a strip
 #define I4_TILE_WORDS 128              // 16 rows x 64 k
 #define I4_CHUNK_K 128                 // k of a chunk
-#define I4_CHUNK_WORDS 256             // a strip's codes of a chunk
+#define I4_CODE_WORDS 256              // a block's codes
+
+// words of a block
+__host__ __device__ constexpr int i4_block_words(int group) { return I4_CODE_WORDS + 16 * (128 / group); }
 
 __host__ __device__ static inline long long i4_strips(long long rows) {
   return (rows + I4_STRIP - 1) / I4_STRIP;

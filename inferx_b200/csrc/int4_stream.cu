@@ -9,24 +9,22 @@
 // or a single matrix with a few rows (E = 1).
 //
 // Mapping: out^T = w . x^T with mma.sync.m16n8k16, sixteen weight rows the M side, eight activation
-// rows the N side.  A warp holds two strips of 16 weight rows (DUAL: a gate strip and the up strip of
-// the same columns) against 8 NT activation rows, so an activation fragment serves both.  Per chunk of
-// 128 k a lane loads 2 x 2 x 16 bytes of codes, turns each word into the A side of one mma with three
-// shifts, four logic operations and four exact subtractions, and multiplies the fp32 sums of each
-// group by the group's scale.  fp32 activations are three bfloat16 terms that are multiplied into the
-// same sums.  The warps of a block split K by chunks and join their sums through shared memory in warp
-// order, so a row's result does not depend on which rows share its tile.
+// rows the N side.  A warp holds S strips of 16 weight rows (DUAL: a gate strip and the up strip of the
+// same columns) against 8 NT activation rows, so an activation fragment serves them all.  Blocks of
+// 128 k come by cp.async into a ring of the warp's own (nobody else reads it: no barrier in the loop),
+// R - 1 of them in flight; the next chunk's activations are loaded ahead into registers.  Each word of
+// codes becomes the A side of one mma by three shifts, four logic operations and four exact
+// subtractions, and the fp32 sums of a group are multiplied by the group's scale.  fp32 activations are
+// three bfloat16 terms, the two small ones summed apart from the first.  The warps of a block split K by
+// chunks and join their sums through shared memory in warp order, so a row's result does not depend on
+// which rows share its tile.
 #include "int4_format.cuh"
 
 #define I4S_THREADS 256
 #define I4S_WARPS 8
 
-__device__ __forceinline__ uint4 i4s_ld16(const unsigned* p) {
-  uint4 r;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
-               : "l"(p));
-  return r;
+__device__ __forceinline__ void i4s_copy16(unsigned to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
 }
 __device__ __forceinline__ void i4s_mma(float* c, const unsigned* a, unsigned b0, unsigned b1) {
   asm volatile(
@@ -34,23 +32,6 @@ __device__ __forceinline__ void i4s_mma(float* c, const unsigned* a, unsigned b0
       "{%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-// NG words (1, 2 or 4) that lie beside each other
-template <int NG> __device__ __forceinline__ void i4s_params(const unsigned* p, unsigned* v) {
-  if (NG == 1) v[0] = __ldg(p);
-  if (NG == 2) {
-    const uint2 r = __ldg(reinterpret_cast<const uint2*>(p));
-    v[0] = r.x;
-    v[NG - 1] = r.y;
-  }
-  if (NG == 4) {
-    const uint4 r = __ldg(reinterpret_cast<const uint4*>(p));
-    v[0] = r.x;
-    v[NG > 1 ? 1 : 0] = r.y;
-    v[NG > 2 ? 2 : 0] = r.z;
-    v[NG - 1] = r.w;
-  }
 }
 
 // Eight activations of a row as fragments: [term][pair of k].
@@ -106,43 +87,65 @@ __device__ __forceinline__ void i4s_store(const I4Out& o, size_t r, int j, int N
   else ((bf16*)o.out)[r * N + j] = __float2bfloat16_rn(v);
 }
 
-template <typename XT, bool DUAL, int NT, int GROUP>
-__global__ void __launch_bounds__(I4S_THREADS)
+template <int NT, int GROUP, int S> struct I4SCfg {
+  static constexpr int BYTES = i4_block_words(GROUP) * 4;          // a strip's share of a chunk
+  static constexpr int R = S == 1 ? 8 : 6;                         // stages of a warp's ring
+  static constexpr int RING = I4S_WARPS * R * S * BYTES;
+  static constexpr int SMEM = RING + S * I4S_WARPS * NT * 128 * 4; // and the sums that are joined
+};
+
+template <typename XT, bool DUAL, int NT, int GROUP, int S>
+__global__ void __launch_bounds__(I4S_THREADS, NT == 1 && sizeof(XT) == 2 ? 2 : 1)
 int4_stream_kernel(const XT* __restrict__ x, const int* __restrict__ rows,
-                   const int* __restrict__ offsets, const unsigned* __restrict__ codes,
-                   const unsigned* __restrict__ params, I4Out out, int M_single, int N, int K,
-                   int strips, int chunks, int ksplit, int offsets_settled) {
-  constexpr int NG = 128 / GROUP, PER = GROUP / 32, D = 2;
-  constexpr int TERMS = I4Frag<XT>::TERMS;
-  __shared__ float red[2][I4S_WARPS][NT][4][32];
+                   const int* __restrict__ offsets, const unsigned* __restrict__ data, I4Out out,
+                   int M_single, int N, int K, int strips, int chunks, int ksplit,
+                   int offsets_settled) {
+  typedef I4SCfg<NT, GROUP, S> C;
+  constexpr int NG = 128 / GROUP, PER = GROUP / 32;
+  constexpr int TERMS = I4Frag<XT>::TERMS, ACCS = TERMS == 3 ? 2 : 1;
+  static_assert(!DUAL || S == 2, "a gate strip and its up strip");
+  extern __shared__ __align__(16) unsigned char smem[];
+  float* red = reinterpret_cast<float*>(smem + C::RING);           // [S][warp][NT][4][32]
   const int e = blockIdx.y;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, t = lane & 3;
   const int tiles = I4S_WARPS / ksplit;
   const int tile = warp / ksplit, ks = warp % ksplit;
   const int pos = blockIdx.x * tiles + tile;
-  // the warp's two strips; where there is none its loads go to the first and are not stored
-  const int s0 = DUAL ? pos : 2 * pos, s1 = DUAL ? pos : 2 * pos + 1;
-  const size_t matrix = (size_t)e * (DUAL ? 2 : 1);
-  const size_t b0 = (matrix * strips + (s0 < strips ? s0 : 0)) * chunks;
-  const size_t b1 = ((matrix + (DUAL ? 1 : 0)) * strips + (s1 < strips ? s1 : 0)) * chunks;
-  const unsigned* cw[2] = {codes + b0 * I4_CHUNK_WORDS + lane * 4,
-                           codes + b1 * I4_CHUNK_WORDS + lane * 4};
-  const unsigned* cp[2] = {params + (b0 * I4_STRIP + g) * NG, params + (b1 * I4_STRIP + g) * NG};
-  uint4 w[D][2][2];
-  unsigned prm[D][2][2][NG];
-  auto fetch_w = [&](int u, int c) {
-    if (c < chunks) {
+  // the warp's strips; where there is none its copies come from the first and are not stored
+  const size_t pitch = (size_t)strips * C::BYTES;                  // from chunk to chunk
+  const unsigned char* base = reinterpret_cast<const unsigned char*>(data) +
+                              (size_t)e * (DUAL ? 2 : 1) * chunks * pitch;
+  const unsigned char* from[S];
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        w[u][s][0] = i4s_ld16(cw[s] + (size_t)c * I4_CHUNK_WORDS);
-        w[u][s][1] = i4s_ld16(cw[s] + (size_t)c * I4_CHUNK_WORDS + I4_TILE_WORDS);
-        i4s_params<NG>(cp[s] + (size_t)c * I4_STRIP * NG, prm[u][s][0]);
-        i4s_params<NG>(cp[s] + ((size_t)c * I4_STRIP + 8) * NG, prm[u][s][1]);
+  for (int s = 0; s < S; ++s) {
+    const int strip = DUAL ? pos : S * pos + s;
+    from[s] = base + (DUAL && s ? chunks * pitch : 0) +
+              (size_t)(strip < strips ? strip : 0) * C::BYTES;
+  }
+  // parameters of a strip: 4 NG pieces of 16 bytes, lanes 0.. for the first strip, 16.. for the second
+  const bool copies_params = (lane & 15) < 4 * NG && (lane >> 4) < S;
+  const unsigned char* from_params =
+      from[S == 2 ? lane >> 4 : 0] + I4_CODE_WORDS * 4 + (lane & 15) * 16;
+  const unsigned params_at = (S == 2 ? (lane >> 4) * C::BYTES : 0) + I4_CODE_WORDS * 4 + (lane & 15) * 16;
+  unsigned char* ring = smem + warp * (C::R * S * C::BYTES);
+  const unsigned ring_at = (unsigned)__cvta_generic_to_shared(ring);
+  const int n = chunks > ks ? (chunks - ks + ksplit - 1) / ksplit : 0;   // chunks of this warp
+  auto fetch = [&](int i) {                        // its i-th chunk, if there is one
+    if (i < n) {
+      const size_t c = (size_t)(ks + i * ksplit) * pitch;
+      const unsigned at = ring_at + (i % C::R) * (S * C::BYTES);
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        i4s_copy16(at + s * C::BYTES + lane * 16, from[s] + c + lane * 16);
+        i4s_copy16(at + s * C::BYTES + I4_TILE_WORDS * 4 + lane * 16,
+                   from[s] + c + I4_TILE_WORDS * 4 + lane * 16);
       }
+      if (copies_params) i4s_copy16(at + params_at, from_params + c);
     }
+    asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  // Weights are never written on the device while steps run: the first loads go out before the
+  // Weights are never written on the device while steps run: the first copies go out before the
   // wait on the predecessor where the range of rows is known already.
   const bool early = offsets == nullptr || offsets_settled != 0;
   int lo = 0, hi = M_single;
@@ -152,8 +155,7 @@ int4_stream_kernel(const XT* __restrict__ x, const int* __restrict__ rows,
       hi = offsets[e + 1];
     }
     if (lo >= hi) return;
-#pragma unroll
-    for (int u = 0; u < D; ++u) fetch_w(u, ks + u * ksplit);
+    for (int i = 0; i < C::R - 1; ++i) fetch(i);
   }
   IX_PDL_WAIT();
   if (!early) {
@@ -171,152 +173,191 @@ int4_stream_kernel(const XT* __restrict__ x, const int* __restrict__ rows,
       const size_t src = xok[i] ? (rows ? (size_t)rows[r] : (size_t)r) : 0;
       xrow[i] = x + src * K + t * 8;
     }
-    float tot[2][NT][4];
+    float tot[S][NT][4];
 #pragma unroll
-    for (int s = 0; s < 2; ++s)
+    for (int s = 0; s < S; ++s)
 #pragma unroll
       for (int i = 0; i < NT; ++i)
 #pragma unroll
         for (int c = 0; c < 4; ++c) tot[s][i][c] = 0.f;
     if (!(early && r0 == lo)) {
-#pragma unroll
-      for (int u = 0; u < D; ++u) fetch_w(u, ks + u * ksplit);
+      __syncwarp();                                // the previous pass has read its parameters
+      for (int i = 0; i < C::R - 1; ++i) fetch(i);
     }
-    for (int c0 = ks; c0 < chunks; c0 += D * ksplit) {
+    I4Frag<XT> f[4][NT], f_next[4][NT];
+    auto fetch_x = [&](int i) {
+      const int k0 = (ks + i * ksplit) * I4_CHUNK_K;
 #pragma unroll
-      for (int u = 0; u < D; ++u) {
-        const int c = c0 + u * ksplit;
-        if (c < chunks) {
-          I4Frag<XT> f[4][NT];
+      for (int b = 0; b < 4; ++b)
 #pragma unroll
-          for (int b = 0; b < 4; ++b)
+        for (int j = 0; j < NT; ++j)
+          f_next[b][j].load(xrow[j] + k0 + b * 32, xok[j] && i < n && k0 + b * 32 + t * 8 < K);
+    };
+    fetch_x(0);
+    for (int i = 0; i < n; ++i) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(C::R - 2) : "memory");
+      __syncwarp();            // parameters were copied by other lanes; the last chunk's are read
+      fetch(i + C::R - 1);
 #pragma unroll
-            for (int i = 0; i < NT; ++i) {
-              const int k = c * I4_CHUNK_K + b * 32;
-              f[b][i].load(xrow[i] + k, xok[i] && k + t * 8 < K);
-            }
-          float acc[2][NT][4];
+      for (int b = 0; b < 4; ++b)
 #pragma unroll
-          for (int b = 0; b < 4; ++b) {
-            if (b % PER == 0) {
+        for (int j = 0; j < NT; ++j) f[b][j] = f_next[b][j];
+      fetch_x(i + 1);
+      const unsigned* block = reinterpret_cast<const unsigned*>(ring + (i % C::R) * (S * C::BYTES));
+      uint4 w[S][2];
+      unsigned pa[S][NG], pb[S][NG];
 #pragma unroll
-              for (int s = 0; s < 2; ++s)
+      for (int s = 0; s < S; ++s) {
+        const unsigned* at = block + s * (C::BYTES / 4);
+        w[s][0] = *reinterpret_cast<const uint4*>(at + lane * 4);
+        w[s][1] = *reinterpret_cast<const uint4*>(at + I4_TILE_WORDS + lane * 4);
 #pragma unroll
-                for (int i = 0; i < NT; ++i)
+        for (int q = 0; q < NG; ++q) {
+          pa[s][q] = at[I4_CODE_WORDS + g * NG + q];
+          pb[s][q] = at[I4_CODE_WORDS + (g + 8) * NG + q];
+        }
+      }
+      float acc[ACCS][S][NT][4];
 #pragma unroll
-                  for (int q = 0; q < 4; ++q) acc[s][i][q] = 0.f;
-            }
-            unsigned a[2][2][4];
+      for (int b = 0; b < 4; ++b) {
+        if (b % PER == 0) {
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-              const uint4 v = w[u][s][b >> 1];
-              const unsigned word[2] = {(b & 1) ? v.z : v.x, (b & 1) ? v.w : v.y};
-              const unsigned sa = i4_sub(prm[u][s][0][b / PER]), sb = i4_sub(prm[u][s][1][b / PER]);
+          for (int a = 0; a < ACCS; ++a)
 #pragma unroll
-              for (int j = 0; j < 2; ++j) {
-                a[s][j][0] = i4_pair(word[j], 0, sa);
-                a[s][j][1] = i4_pair(word[j], 1, sb);
-                a[s][j][2] = i4_pair(word[j], 2, sa);
-                a[s][j][3] = i4_pair(word[j], 3, sb);
-              }
-            }
+            for (int s = 0; s < S; ++s)
 #pragma unroll
-            for (int i = 0; i < NT; ++i) {
-              unsigned xb[TERMS][4];
-              f[b][i].terms(xb);
+              for (int j = 0; j < NT; ++j)
 #pragma unroll
-              for (int m = 0; m < TERMS; ++m)
+                for (int q = 0; q < 4; ++q) acc[a][s][j][q] = 0.f;
+        }
+        unsigned a[S][2][4];
 #pragma unroll
-                for (int s = 0; s < 2; ++s) {
-                  i4s_mma(acc[s][i], a[s][0], xb[m][0], xb[m][1]);
-                  i4s_mma(acc[s][i], a[s][1], xb[m][2], xb[m][3]);
-                }
-            }
-            if (b % PER == PER - 1) {
+        for (int s = 0; s < S; ++s) {
+          const uint4 v = w[s][b >> 1];
+          const unsigned word[2] = {(b & 1) ? v.z : v.x, (b & 1) ? v.w : v.y};
+          const unsigned sa = i4_sub(pa[s][b / PER]), sb = i4_sub(pb[s][b / PER]);
 #pragma unroll
-              for (int s = 0; s < 2; ++s) {
-                const float fa = i4_scale(prm[u][s][0][b / PER]);
-                const float fb = i4_scale(prm[u][s][1][b / PER]);
-#pragma unroll
-                for (int i = 0; i < NT; ++i) {
-                  tot[s][i][0] = fmaf(fa, acc[s][i][0], tot[s][i][0]);
-                  tot[s][i][1] = fmaf(fa, acc[s][i][1], tot[s][i][1]);
-                  tot[s][i][2] = fmaf(fb, acc[s][i][2], tot[s][i][2]);
-                  tot[s][i][3] = fmaf(fb, acc[s][i][3], tot[s][i][3]);
-                }
-              }
-            }
+          for (int j = 0; j < 2; ++j) {
+            a[s][j][0] = i4_pair(word[j], 0, sa);
+            a[s][j][1] = i4_pair(word[j], 1, sb);
+            a[s][j][2] = i4_pair(word[j], 2, sa);
+            a[s][j][3] = i4_pair(word[j], 3, sb);
           }
         }
-        fetch_w(u, c + D * ksplit);
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          unsigned xb[TERMS][4];
+          f[b][j].terms(xb);
+#pragma unroll
+          for (int m = TERMS - 1; m >= 0; --m)
+#pragma unroll
+            for (int s = 0; s < S; ++s) {
+              float* sum = acc[m > 0 ? ACCS - 1 : 0][s][j];
+              i4s_mma(sum, a[s][0], xb[m][0], xb[m][1]);
+              i4s_mma(sum, a[s][1], xb[m][2], xb[m][3]);
+            }
+        }
+        if (b % PER == PER - 1) {
+#pragma unroll
+          for (int s = 0; s < S; ++s) {
+            const float fa = i4_scale(pa[s][b / PER]), fb = i4_scale(pb[s][b / PER]);
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                float v = acc[0][s][j][q];
+                if (ACCS == 2) v += acc[ACCS - 1][s][j][q];
+                tot[s][j][q] = fmaf(q < 2 ? fa : fb, v, tot[s][j][q]);
+              }
+          }
+        }
       }
     }
-    // c0, c1: column g of the strip, rows 2t and 2t + 1; c2, c3: column g + 8
+    // q = 0, 1: column g of the strip, rows 2t and 2t + 1; q = 2, 3: column g + 8
+    auto store = [&](int p, int col, int r, float v, float u) {
+      if (r >= hi) return;
+      const int j = (DUAL ? p : S * p) * I4_STRIP + col;
+      if (j < N) i4s_store<DUAL>(out, r, j, N, v, u);
+      if (S == 2 && !DUAL && j + I4_STRIP < N) i4s_store<DUAL>(out, r, j + I4_STRIP, N, u, 0.f);
+    };
     if (ksplit == 1) {
 #pragma unroll
-      for (int i = 0; i < NT; ++i)
+      for (int j = 0; j < NT; ++j)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const int col = (c & 2) ? g + 8 : g;
-          const int r = r0 + i * 8 + 2 * t + (c & 1);
-          if (r >= hi) continue;
-          if (s0 * I4_STRIP + col < N)
-            i4s_store<DUAL>(out, r, s0 * I4_STRIP + col, N, tot[0][i][c], tot[1][i][c]);
-          if (!DUAL && s1 * I4_STRIP + col < N)
-            i4s_store<DUAL>(out, r, s1 * I4_STRIP + col, N, tot[1][i][c], 0.f);
-        }
+        for (int q = 0; q < 4; ++q)
+          store(pos, (q & 2) ? g + 8 : g, r0 + j * 8 + 2 * t + (q & 1), tot[0][j][q],
+                tot[S - 1][j][q]);
     } else {
       __syncthreads();   // the previous pass has read its sums
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
+      for (int s = 0; s < S; ++s)
 #pragma unroll
-        for (int i = 0; i < NT; ++i)
+        for (int j = 0; j < NT; ++j)
 #pragma unroll
-          for (int c = 0; c < 4; ++c) red[s][warp][i][c][lane] = tot[s][i][c];
+          for (int q = 0; q < 4; ++q)
+            red[(((s * I4S_WARPS + warp) * NT + j) * 4 + q) * 32 + lane] = tot[s][j][q];
       __syncthreads();
       for (int idx = threadIdx.x; idx < tiles * NT * 128; idx += I4S_THREADS) {
-        const int l = idx & 31, c = (idx >> 5) & 3, i = (idx >> 7) % NT, ti = idx / (NT * 128);
-        float v = 0.f, v2 = 0.f;
-        for (int q = 0; q < ksplit; ++q) {
-          v += red[0][ti * ksplit + q][i][c][l];
-          v2 += red[1][ti * ksplit + q][i][c][l];
+        const int l = idx & 31, q = (idx >> 5) & 3, j = (idx >> 7) % NT, ti = idx / (NT * 128);
+        float v = 0.f, u = 0.f;
+        for (int k = 0; k < ksplit; ++k) {
+          const int at = ((ti * ksplit + k) * NT + j) * 128 + q * 32 + l;
+          v += red[at];
+          if (S == 2) u += red[I4S_WARPS * NT * 128 + at];
         }
-        const int p = blockIdx.x * tiles + ti;
-        const int col = (l >> 2) + ((c & 2) ? 8 : 0);
-        const int r = r0 + i * 8 + 2 * (l & 3) + (c & 1);
-        if (r >= hi) continue;
-        const int j0 = (DUAL ? p : 2 * p) * I4_STRIP + col;
-        if (j0 < N) i4s_store<DUAL>(out, r, j0, N, v, v2);
-        if (!DUAL && j0 + I4_STRIP < N) i4s_store<DUAL>(out, r, j0 + I4_STRIP, N, v2, 0.f);
+        store(blockIdx.x * tiles + ti, (l >> 2) + ((q & 2) ? 8 : 0),
+              r0 + j * 8 + 2 * (l & 3) + (q & 1), v, u);
       }
     }
   }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
-template <typename XT, bool DUAL, int NT, int GROUP>
-static int i4s_launch(const void* x, const int* rows, const int* offsets, const void* codes,
-                      const void* params, I4Out out, int M, int N, int K, int E, int active,
-                      int settled, cudaStream_t stream) {
-  const int strips = (int)i4_strips(N), chunks = (int)i4_chunks(K);
-  const int pairs = DUAL ? strips : (strips + 1) / 2;
-  // K is split over the warps of a block until every SM has eight warps
+struct I4SCall {
+  const void* x;
+  const int *rows, *offsets;
+  const void* data;
+  I4Out out;
+  int M, N, K, E, active, settled;
+};
+
+template <typename XT, bool DUAL, int NT, int GROUP, int S>
+static int i4s_launch2(const I4SCall& c, cudaStream_t stream) {
+  typedef I4SCfg<NT, GROUP, S> C;
+  const int strips = (int)i4_strips(c.N), chunks = (int)i4_chunks(c.K);
+  const int sets = DUAL ? strips : (strips + S - 1) / S;
+  // K is split over the warps of a block until every SM has sixteen warps
   int ksplit = 1;
-  while (ksplit < 8 && ksplit < chunks && (long long)pairs * active * ksplit < 148 * 8) ksplit *= 2;
+  while (ksplit < 8 && ksplit < chunks && (long long)sets * c.active * ksplit < 148 * 16) ksplit *= 2;
   const int tiles = I4S_WARPS / ksplit;
-  ix_launch(int4_stream_kernel<XT, DUAL, NT, GROUP>, dim3((pairs + tiles - 1) / tiles, E),
-            dim3(I4S_THREADS), 0, stream, (const XT*)x, rows, offsets, (const unsigned*)codes,
-            (const unsigned*)params, out, offsets ? 0 : M, N, K, strips, chunks, ksplit, settled);
+  auto kern = int4_stream_kernel<XT, DUAL, NT, GROUP, S>;
+  const cudaError_t e =
+      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+  if (e != cudaSuccess) return (int)e;
+  ix_launch(kern, dim3((sets + tiles - 1) / tiles, c.E), dim3(I4S_THREADS), C::SMEM, stream,
+            (const XT*)c.x, c.rows, c.offsets, (const unsigned*)c.data, c.out, c.offsets ? 0 : c.M,
+            c.N, c.K, strips, chunks, ksplit, c.settled);
   return ix_launch_status();
 }
 
-// x: [*, K] fp32 or bf16, K a multiple of 8, 16-byte aligned; codes and params as int4_format.cuh
-// lays them out, [E or 2 E matrices]; out: [rows, N] fp32 (wide) or bf16.  offsets == null: one
+template <typename XT, bool DUAL, int NT, int GROUP>
+static int i4s_launch(const I4SCall& c, cudaStream_t stream) {
+  if constexpr (!DUAL) {
+    // one strip a warp while pairs of them would not reach every SM
+    if (i4_strips(c.N) * c.active < 2 * 148 * 2)
+      return i4s_launch2<XT, false, NT, GROUP, 1>(c, stream);
+  }
+  return i4s_launch2<XT, DUAL, NT, GROUP, 2>(c, stream);
+}
+
+// x: [*, K] fp32 or bf16, K a multiple of 8, 16-byte aligned; data as int4_format.cuh lays
+// it out, [E or 2 E matrices]; out: [rows, N] fp32 (wide) or bf16.  offsets == null: one
 // matrix with M rows.  active: how many of the E groups are expected to have rows.
 // offsets_settled: nonzero when `offsets` was written at least two launches back in the stream.
 IX_API int ix_int4_stream(const void* x, int x_dtype, const int* rows, const int* offsets,
-                          const void* codes, const void* params, void* out, int wide, int dual,
-                          int M, int N, int K, int E, int group, int rows_per_pass, int active,
-                          int offsets_settled, const float* row_scale, int plain,
+                          const void* data, void* out, int wide, int dual, int M, int N, int K, int E,
+                          int group, int rows_per_pass, int active, int offsets_settled,
+                          const float* row_scale, int plain,
                           cudaStream_t stream) {
   if ((row_scale && !dual) || (plain && dual)) return IX_ERR_UNSUPPORTED;
   if (N <= 0 || K <= 0 || E <= 0 || E > 65535) return IX_ERR_SIZE;
@@ -325,10 +366,10 @@ IX_API int ix_int4_stream(const void* x, int x_dtype, const int* rows, const int
   if (!offsets && M <= 0) return IX_OK;
   if ((uintptr_t)x & 15) return IX_ERR_ALIGN;
   if (active <= 0 || active > E) active = E;
-  const I4Out o = {out, wide, row_scale, plain};
+  const I4SCall c = {x, rows, offsets, data, {out, wide, row_scale, plain}, M, N, K, E, active,
+                     offsets_settled};
   const int nt = rows_per_pass > 16 ? 4 : rows_per_pass > 8 ? 2 : 1;
-#define I4S_GO(T, D, NT, G) \
-  return i4s_launch<T, D, NT, G>(x, rows, offsets, codes, params, o, M, N, K, E, active, offsets_settled, stream)
+#define I4S_GO(T, D, NT, G) return i4s_launch<T, D, NT, G>(c, stream)
 // (32 rows of three terms each would not fit the registers: fp32 takes 16 a pass)
 #define I4S_NT(T, D, G)                                             \
   do {                                                              \

@@ -7,90 +7,186 @@
 // `a` holds bfloat16 rows grouped by expert (offsets), or the rows of a single matrix; fp32 rows come
 // as three planes of bfloat16 terms that are multiplied into the same sums.
 //
-// The weights are the M side of tcgen05.mma and the rows the N side.  An item of work is 128 weight
-// rows (DUAL: 64 gate rows and the up rows of the same columns) for a tile of up to BT rows of one
-// expert; blocks are persistent, one per SM, and take items round robin, the weight tiles of one row
-// tile beside each other.  Roles:
-//   warp 0      brings the rows, 64 k at a time, into a ring of stages (TMA, 128-byte swizzle);
-//   warp 1      issues the MMAs, a group of k into one of two accumulators in tensor memory;
-//   warps 2-9   load their strip's codes straight into registers (a lane's 16 bytes are eight
-//               neighbouring k of two rows, twice), subtract the zero points, and write whole numbers
-//               as a swizzled operand tile into a ring of their own; and take each finished group's
-//               sums out of tensor memory, a weight row a lane, and add scale * sum to fp32 registers.
-// So the operands of the tensor cores are exact (a code less its zero point has five bits), sums of a
-// group are the tensor cores' fp32, and a group's scale multiplies in fp32: no weight is rounded to
-// bfloat16.  The warps unpack the next chunk of 128 k before they take the sums of the last one, also
-// across items, so the MMAs run meanwhile.
+// The weights are the M side of tcgen05.mma and the rows the N side.  Two SMs work on one item
+// (cta_group::2): 256 weight rows (DUAL: 128 gate rows and the up rows of the same columns) for a tile
+// of up to BT rows of one expert, over all of K or one of `splits` runs of it.  A block holds 128 of the
+// weight rows and half of the tile's rows, so each of the two halves is brought once.  Pairs are
+// persistent and take items round robin.  Roles of a block's sixteen warps, a chunk of 128 k at a time:
+//   0      brings the rows into a ring of stages (TMA, 128-byte swizzle);
+//   1      the first block's issues the MMAs for both, a group of k into one of two accumulators in
+//          tensor memory; the second block's tells the first that its own operands are there;
+//   2      brings the codes and parameters of the block's eight strips (one bulk copy, DUAL two);
+//   4-11   take each finished group's sums out of tensor memory, a weight row a lane, and add scale *
+//          sum to fp32 registers;
+//          Rows of a DUAL item lie as 16 gate rows, the 16 up rows of the same columns, and so on, so
+//          that a column's two sums are sixteen lanes of one warp apart;
+//   12-15  unpack: a lane's 16 bytes of codes are eight neighbouring k of two rows, twice; less their
+//          zero points they are whole numbers, written as a swizzled operand tile.
+// So the operands of the tensor cores are exact (a code less its zero point has five bits), the sums of
+// a group are the tensor cores' fp32, and a group's scale multiplies in fp32: no weight is rounded to
+// bfloat16.
 //
 // Columns past the tile and weight rows past N are computed on whatever is there and never stored.
-// Every wait on an mbarrier is bounded: the waiter records a code in `status` (51 copies, 52 MMAs, 53
-// the unpacking warps), raises a flag that ends the other roles, and the block frees its tensor memory.
+// Every wait on an mbarrier is bounded: the waiter records a code in `status` (51 and 54 copies, 52
+// MMAs, 53 unpacking, 55 sums), raises a flag that ends its block's other roles, and the pair meets at
+// its end, where tensor memory is freed.
 #include "int4_format.cuh"
 #include "tcgen05_common.cuh"
 #include "tma_common.cuh"
 
-#define I4T_THREADS 320
-#define I4T_WORKERS 8
-#define I4T_BOX 32                        // rows of a TMA box
-#define I4T_A_BYTES (128 * 64 * 2)        // an operand tile of weights
+#define I4T_THREADS 512
+#define I4T_TILE (128 * 64 * 2)           // 64 k of a block's weight rows, unpacked
 #define I4T_MAX_EXPERTS 1024              // the prefix of tiles lives in shared memory
-#define I4T_EXCHANGE (4 * 32 * 33 * 4)    // DUAL: up sums on their way to the gate's warps
+#define I4T_DONE 4                        // barriers of finished chunks
 
-enum { I4T_ERR_COPY = 51, I4T_ERR_MMA = 52, I4T_ERR_WORK = 53 };
+enum {
+  I4T_ERR_COPY = 51, I4T_ERR_MMA = 52, I4T_ERR_UNPACK = 53, I4T_ERR_CODES = 54, I4T_ERR_SUM = 55
+};
 
 struct I4TArgs {
   const int* offsets;       // null: one matrix with `rows` rows
-  const unsigned* codes;
-  const unsigned* params;
+  const unsigned* data;
   void* out;
+  float* part;              // splits > 1: [splits][rows][columns of both halves] sums
   int wide;                 // fp32 results, otherwise bfloat16
   const float* row_scale;
   int plain;
   int rows, N, strips, chunks, E;
-  int tile_rows;            // one matrix: rows of a tile, a multiple of 16
+  int tile_rows;            // one matrix: rows of a tile, a multiple of 32
+  int splits, run;          // runs of K, chunks of a run
   int plane_rows;           // rows of one plane of terms
   int* status;
 };
 
 struct I4TItem {
-  int e, m0, n, f0;
+  int e, m0, n, f0, c0, c1, z;
 };
 
 template <int TERMS, bool DUAL, int BT, int GROUP> struct I4TCfg {
-  static constexpr int X_BYTES = BT * 64 * 2;                  // a term's rows of a stage
-  static constexpr int A_RING = TERMS == 3 ? 3 : 4;
-  static constexpr int X_RING = TERMS == 3 ? 3 : BT == 256 ? 4 : 6;
-  static constexpr int SMEM = X_RING * TERMS * X_BYTES + A_RING * I4T_A_BYTES +
-                              (DUAL ? I4T_EXCHANGE : 0) + 1024;
+  static constexpr int X_TILE = BT / 2 * 64 * 2;               // 64 k of a block's rows, one term
+  static constexpr int X_STAGE = TERMS * 2 * X_TILE;
+  static constexpr int BOX = BT / 4;                           // rows of a TMA box
+  static constexpr int C_BYTES = i4_block_words(GROUP) * 4;    // a strip's codes and parameters
+  static constexpr int X_RING = TERMS == 3 ? 2 : 4;
+  static constexpr int A_RING = BT == 128 && TERMS == 1 ? 3 : 2;
+  static constexpr int C_RING = BT == 128 ? 4 : 2;
+  // Scales are written once the MMAs of A_RING chunks before have run, and those had waited for the
+  // sums of two chunks before them to be taken: a slot is read by then.
+  static constexpr int S_RING = A_RING + 2;
+  static constexpr int SMEM = X_RING * X_STAGE + A_RING * 2 * I4T_TILE + C_RING * 8 * C_BYTES +
+                              S_RING * 128 * (128 / GROUP) * 2 + 1024;
+  static_assert(SMEM + 4608 <= 227 * 1024, "shared memory");
+  static_assert(X_RING <= I4T_DONE && A_RING <= I4T_DONE, "a stage's last use is still to be seen");
   static constexpr unsigned TMEM_COLS = 2 * BT;
-  static constexpr int F = DUAL ? 64 : 128;                    // output columns of an item
+  static constexpr int F = DUAL ? 128 : 256;                   // output columns of an item
 };
+
+// bytes (a multiple of 16, both sides 16-byte aligned) into shared memory, counted at `bar`
+__device__ __forceinline__ void i4t_copy(void* to, const void* from, unsigned bytes,
+                                         unsigned long long* bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+          smem_u32(to)),
+      "l"(from), "r"(bytes), "r"(smem_u32(bar))
+      : "memory");
+}
+// mbar_wait for what the other block of the pair has written.  (A fence.acq_rel.cluster behind a wait
+// of the block's own scope took 1,000 cycles a chunk.)
+__device__ __forceinline__ bool i4t_wait_cluster(unsigned long long* bar, unsigned parity,
+                                                 volatile int* abort_flag) {
+  for (int i = 0; i < IX_WAIT_POLLS; ++i) {
+    unsigned ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    if (ok) return true;
+    if (*abort_flag) return false;
+    if (i > 1024) __nanosleep(64);
+  }
+  return false;
+}
+// two fp32 numbers as one 64-bit register, and a * b + c on both
+__device__ __forceinline__ unsigned long long i4t_pack(float a, float b) {
+  unsigned long long r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void i4t_unpack(unsigned long long v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ void i4t_fma2(unsigned long long& c, unsigned long long a,
+                                         unsigned long long b) {
+  asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(c) : "l"(a), "l"(b));
+}
+
+// the low halves of NG parameters beside each other
+template <int NG> __device__ __forceinline__ void i4t_scales(unsigned short* to, const unsigned* v) {
+  if (NG == 1) *to = (unsigned short)v[0];
+  if (NG == 2) *reinterpret_cast<unsigned*>(to) = __byte_perm(v[0], v[NG - 1], 0x5410);
+  if (NG == 4)
+    *reinterpret_cast<uint2*>(to) =
+        make_uint2(__byte_perm(v[0], v[NG > 1 ? 1 : 0], 0x5410),
+                   __byte_perm(v[NG > 2 ? 2 : 0], v[NG - 1], 0x5410));
+}
+// Out of line: an epilogue that holds them unrolled runs from a cold instruction cache.
+__device__ __noinline__ float i4t_act(float v, int act, int wide) {
+  return wide ? ix_act<float>(v, act) : ix_act<bf16>(v, act);
+}
+__device__ __noinline__ float i4t_silu_wide(float a, float u) { return a / (1.0f + expf(-a)) * u; }
+
+// Up to ROWS rows of one column (the first at entry `at` of the result).
+template <int ROWS>
+__device__ __forceinline__ void i4t_store(const I4TArgs& p, float* v, int n, size_t at) {
+  if (p.plain) {
+#pragma unroll
+    for (int j = 0; j < ROWS; ++j) v[j] = i4t_act(v[j], p.plain, p.wide);
+  }
+  if (p.wide) {
+    float* o = (float*)p.out + at;
+#pragma unroll
+    for (int j = 0; j < ROWS; ++j)
+      if (j < n) o[(size_t)j * p.N] = v[j];
+  } else {
+    bf16* o = (bf16*)p.out + at;
+#pragma unroll
+    for (int j = 0; j < ROWS; ++j)
+      if (j < n) o[(size_t)j * p.N] = __float2bfloat16_rn(v[j]);
+  }
+}
 
 template <int BT>
 __device__ __forceinline__ int i4t_tiles(int rows) { return (rows + BT - 1) / BT; }
 
 template <int TERMS, bool DUAL, int BT, int GROUP>
-__global__ void __launch_bounds__(I4T_THREADS, 1)
-int4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const I4TArgs p) {
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I4T_THREADS, 1)
+int4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ I4TArgs p) {
   typedef I4TCfg<TERMS, DUAL, BT, GROUP> C;
   constexpr int NG = 128 / GROUP;
   constexpr int F = C::F;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* xs =
       reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  unsigned char* as = xs + C::X_RING * TERMS * C::X_BYTES;
-  float* exchange = reinterpret_cast<float*>(as + C::A_RING * I4T_A_BYTES);
-  __shared__ __align__(8) unsigned long long full_x[C::X_RING], empty_x[C::X_RING];
-  __shared__ __align__(8) unsigned long long full_a[C::A_RING], empty_a[C::A_RING];
+  unsigned char* as = xs + C::X_RING * C::X_STAGE;
+  unsigned char* cs = as + C::A_RING * 2 * I4T_TILE;
+  unsigned short* scales = reinterpret_cast<unsigned short*>(cs + C::C_RING * 8 * C::C_BYTES);
+  __shared__ __align__(8) unsigned long long full_x[C::X_RING], full_a[C::A_RING];
+  __shared__ __align__(8) unsigned long long full_c[C::C_RING], empty_c[C::C_RING];
+  __shared__ __align__(8) unsigned long long done[I4T_DONE];     // a chunk's MMAs have run
+  __shared__ __align__(8) unsigned long long full_s[C::S_RING];  // a chunk's scales are there
   __shared__ __align__(8) unsigned long long acc_full[2], acc_empty[2];
-  __shared__ __align__(8) unsigned long long ex_full[4], ex_empty[4];
+  __shared__ __align__(8) unsigned long long peer[4];            // the second block is ready for a group
   __shared__ unsigned tmem_holder;
   __shared__ int abort_flag;
   __shared__ int tile_start[I4T_MAX_EXPERTS + 1];
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const int rank = (int)tc_rank();
   const int f_tiles = (p.N + F - 1) / F;
-  if (warp == 2) {                           // tiles before each expert
+  if (warp == 3) {                           // tiles before each expert
     if (p.offsets) {
       int carry = 0;
       for (int e0 = 0; e0 < p.E; e0 += 32) {
@@ -112,38 +208,41 @@ int4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const I4TArgs p) {
     }
   }
   if (threadIdx.x == 0) {
-    for (int s = 0; s < C::X_RING; ++s) {
-      mbar_init(&full_x[s], 1);
-      mbar_init(&empty_x[s], 1);
+    for (int s = 0; s < C::X_RING; ++s) mbar_init(&full_x[s], 1);
+    for (int s = 0; s < C::A_RING; ++s) mbar_init(&full_a[s], 4);
+    for (int s = 0; s < C::C_RING; ++s) {
+      mbar_init(&full_c[s], 1);
+      mbar_init(&empty_c[s], 4);
     }
-    for (int s = 0; s < C::A_RING; ++s) {
-      mbar_init(&full_a[s], I4T_WORKERS);
-      mbar_init(&empty_a[s], 1);
-    }
+    for (int s = 0; s < I4T_DONE; ++s) mbar_init(&done[s], 1);
+    for (int s = 0; s < C::S_RING; ++s) mbar_init(&full_s[s], 4);
     for (int b = 0; b < 2; ++b) {
       mbar_init(&acc_full[b], 1);
-      mbar_init(&acc_empty[b], I4T_WORKERS);
+      mbar_init(&acc_empty[b], 8);
     }
-    for (int b = 0; b < 4; ++b) {
-      mbar_init(&ex_full[b], 1);
-      mbar_init(&ex_empty[b], 1);
-    }
+    for (int b = 0; b < 4; ++b) mbar_init(&peer[b], 1);
     abort_flag = 0;
     mbar_init_fence();
     fence_proxy_async();
   }
-  if (warp == 1) tc_alloc<false>(&tmem_holder, C::TMEM_COLS);
+  if (warp == 1) tc_alloc<true>(&tmem_holder, C::TMEM_COLS);
   tc_fence_before();
   __syncthreads();
+  tc_cluster_sync();
   tc_fence_after();
   const unsigned tmem_base = __shfl_sync(0xffffffffu, tmem_holder, 0);
   volatile int* abortp = &abort_flag;
-  const int n_items = tile_start[p.E] * f_tiles;
+  const int n_items = tile_start[p.E] * f_tiles * p.splits;
+  const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
 
   auto item_of = [&](int w) {
-    const int tt = w / f_tiles;
     I4TItem it;
+    it.z = w % p.splits;
+    w /= p.splits;
+    const int tt = w / f_tiles;
     it.f0 = (w - tt * f_tiles) * F;
+    it.c0 = it.z * p.run;
+    it.c1 = min(p.chunks, it.c0 + p.run);
     if (p.offsets) {
       int lo = 0, hi = p.E;                  // the last e with tile_start[e] <= tt
       while (hi - lo > 1) {
@@ -153,7 +252,7 @@ int4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const I4TArgs p) {
       it.e = lo;
       const int r0 = p.offsets[lo], rows = p.offsets[lo + 1] - r0;
       const int cuts = i4t_tiles<BT>(rows);
-      const int per = ((rows + cuts - 1) / cuts + 15) & ~15;
+      const int per = ((rows + cuts - 1) / cuts + 31) & ~31;
       it.m0 = r0 + (tt - tile_start[lo]) * per;
       it.n = max(0, min(r0 + rows - it.m0, per));
     } else {
@@ -165,193 +264,247 @@ int4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const I4TArgs p) {
     it.m0 = __shfl_sync(0xffffffffu, it.m0, 0);
     it.n = __shfl_sync(0xffffffffu, it.n, 0);
     it.f0 = __shfl_sync(0xffffffffu, it.f0, 0);
+    it.c0 = __shfl_sync(0xffffffffu, it.c0, 0);
+    it.c1 = __shfl_sync(0xffffffffu, it.c1, 0);
     return it;
   };
+  auto wait = [&](unsigned long long* bar, int parity) {
+    return (bool)__all_sync(0xffffffffu, mbar_wait(bar, parity, abortp));
+  };
 
-  if (warp == 0) {
-    int fill = 0;
-    bool ok = true;
-    for (int w = blockIdx.x; w < n_items && ok; w += gridDim.x) {
-      const I4TItem it = item_of(w);
-      if (it.n <= 0) continue;
-      const int boxes = (((it.n + 15) & ~15) + I4T_BOX - 1) / I4T_BOX;
-      const unsigned tx = (unsigned)(TERMS * boxes * I4T_BOX * 64 * 2);
-      for (int kt = 0; kt < 2 * p.chunks; ++kt, ++fill) {
-        const int s = fill % C::X_RING;
-        ok = __all_sync(0xffffffffu, mbar_wait(&empty_x[s], ((fill / C::X_RING) & 1) ^ 1, abortp));
-        if (!ok) break;
-        if (lane == 0) {
-          mbar_expect_tx(&full_x[s], tx);
-          for (int t = 0; t < TERMS; ++t)
-            for (int b = 0; b < boxes; ++b)
-              tma_load_2d(xs + (s * TERMS + t) * C::X_BYTES + b * (I4T_BOX * 64 * 2), &map_x,
-                          kt * 64, t * p.plane_rows + it.m0 + b * I4T_BOX, &full_x[s]);
+  // Registers go from the roles that need few to the warps that hold up to 128 sums a lane (512
+  // threads at 128: 128 x 40 + 256 x 200 + 128 x 72).
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    if (warp == 0) {
+      int n = 0;                             // chunks so far, over all items
+      bool ok = true;
+      for (int w = first; w < n_items && ok; w += step) {
+        const I4TItem it = item_of(w);
+        if (it.n <= 0) continue;
+        const int half = ((it.n + 31) & ~31) / 2;              // rows of this block
+        const int boxes = (half + C::BOX - 1) / C::BOX;
+        // a lane a box: term, 64 k, 32 rows
+        const int box = lane % boxes, sub = lane / boxes & 1, term = lane / (2 * boxes);
+        for (int c = it.c0; c < it.c1; ++c, ++n) {
+          const int s = n % C::X_RING;
+          if (n >= C::X_RING) {
+            const int before = n - C::X_RING;
+            ok = wait(&done[before % I4T_DONE], before / I4T_DONE & 1);
+            if (!ok) break;
+          }
+          if (lane == 0)
+            mbar_expect_tx(&full_x[s], (unsigned)(TERMS * 2 * boxes * C::BOX * 64 * 2));
+          __syncwarp();
+          if (term < TERMS)
+            tma_load_2d(xs + s * C::X_STAGE + (term * 2 + sub) * C::X_TILE +
+                            box * (C::BOX * 64 * 2),
+                        &map_x, c * 128 + sub * 64,
+                        term * p.plane_rows + it.m0 + rank * half + box * C::BOX, &full_x[s]);
+          __syncwarp();
         }
-        __syncwarp();
       }
-    }
-    if (!ok && lane == 0) {
-      if (!*abortp) { atomicExch(p.status, I4T_ERR_COPY); *abortp = 1; }
-      // copies in flight land before the block's shared memory goes away
-      for (int f = max(0, fill - C::X_RING); f < fill; ++f)
-        mbar_drain(&full_x[f % C::X_RING], (f / C::X_RING) & 1);
-    }
-  } else if (warp == 1) {
-    int tile = 0, group = 0;                 // tiles of 64 k and groups so far, over all items
-    bool ok = true;
-    for (int w = blockIdx.x; w < n_items && ok; w += gridDim.x) {
-      const I4TItem it = item_of(w);
-      if (it.n <= 0) continue;
-      // kind::f16: fp32 sums, both sides bfloat16 and K-major, M 128, N the tile's rows in sixteens
-      const unsigned idesc = (1u << 4) | (1u << 7) | (1u << 10) |
-                             ((unsigned)(((it.n + 15) & ~15) >> 3) << 17) | (8u << 24);
-      for (int kt = 0; kt < 2 * p.chunks && ok; ++kt, ++tile) {
-        const int sx = tile % C::X_RING, sa = tile % C::A_RING;
-        ok = __all_sync(0xffffffffu, mbar_wait(&full_a[sa], (tile / C::A_RING) & 1, abortp)) &&
-             __all_sync(0xffffffffu, mbar_wait(&full_x[sx], (tile / C::X_RING) & 1, abortp));
-        if (!ok) break;
-        tc_fence_after();
-#pragma unroll
-        for (int k4 = 0; k4 < 4; ++k4) {
-          const int at = (kt & 1) * 4 + k4;            // sixteens of k into the chunk
-          const bool first = at % (GROUP / 16) == 0, last = at % (GROUP / 16) == GROUP / 16 - 1;
-          const int buf = group & 1;
-          if (first) {
-            ok = __all_sync(0xffffffffu,
-                            mbar_wait(&acc_empty[buf], ((group >> 1) & 1) ^ 1, abortp));
+      if (lane == 0) {
+        if (!ok && !*abortp) { atomicExch(p.status, I4T_ERR_COPY); *abortp = 1; }
+        // copies in flight land before the block's shared memory goes away, whatever the others do
+        for (int f = max(0, n - C::X_RING); f < n; ++f)
+          mbar_drain(&full_x[f % C::X_RING], f / C::X_RING & 1);
+      }
+    } else if (warp == 1) {
+      const unsigned peer_at = tc_of_rank(&peer[0], 0);
+      int n = 0, group = 0;
+      bool ok = true;
+      for (int w = first; w < n_items && ok; w += step) {
+        const I4TItem it = item_of(w);
+        if (it.n <= 0) continue;
+        // kind::f16: fp32 sums, both sides bfloat16 and K-major, M 256, N the tile's rows
+        const unsigned idesc = (1u << 4) | (1u << 7) | (1u << 10) |
+                               ((unsigned)(((it.n + 31) & ~31) >> 3) << 17) | (16u << 24);
+        for (int c = it.c0; c < it.c1 && ok; ++c, ++n) {
+          const int sx = n % C::X_RING, sa = n % C::A_RING;
+          ok = wait(&full_a[sa], n / C::A_RING & 1) && wait(&full_x[sx], n / C::X_RING & 1);
+          if (!ok) break;
+          const unsigned long long ad = umma_desc(as + sa * 2 * I4T_TILE);
+          const unsigned long long xd = umma_desc(xs + sx * C::X_STAGE);
+          for (int q = 0; q < NG && ok; ++q, ++group) {
+            const int buf = group & 1;
+            ok = wait(&acc_empty[buf], (group >> 1 & 1) ^ 1);
+            if (!ok) break;
+            if (rank != 0) {
+              if (lane == 0) tc_arrive_at(peer_at + (group & 3) * 8);
+              __syncwarp();
+              continue;
+            }
+            ok = (bool)__all_sync(0xffffffffu,
+                                  i4t_wait_cluster(&peer[group & 3], group >> 2 & 1, abortp));
             if (!ok) break;
             tc_fence_after();
-          }
-          if (lane == 0) {
-            const unsigned long long ad = umma_desc(as + sa * I4T_A_BYTES) + 2 * k4;
+            const unsigned sums = tmem_base + buf * BT;
+            if (lane == 0) {
 #pragma unroll
-            for (int t = TERMS - 1; t >= 0; --t)       // small terms first
-              tc_mma(tmem_base + buf * BT, ad,
-                     umma_desc(xs + (sx * TERMS + t) * C::X_BYTES) + 2 * k4, idesc,
-                     (first && t == TERMS - 1) ? 0u : 1u);
-            if (last) tc_commit(&acc_full[buf]);
-            if (k4 == 3) {
-              tc_commit(&empty_a[sa]);
-              tc_commit(&empty_x[sx]);
+              for (int i = 0; i < GROUP / 16; ++i) {
+                // sixteens of k into the chunk; 32 bytes each inside a tile's swizzled rows
+                const int at = q * (GROUP / 16) + i;
+                const unsigned long long a = ad + (at >> 2) * (I4T_TILE >> 4) + (at & 3) * 2;
+#pragma unroll
+                for (int t = TERMS - 1; t >= 0; --t)           // small terms first
+                  tc_mma_pair(sums, a,
+                              xd + (t * 2 + (at >> 2)) * (C::X_TILE >> 4) + (at & 3) * 2, idesc,
+                              i == 0 && t == TERMS - 1 ? 0u : 1u);
+              }
+              if (NG > 1) tc_commit_pair(&acc_full[buf]);
+              if (q == NG - 1) tc_commit_pair(&done[n % I4T_DONE]);
+            }
+            __syncwarp();
+          }
+        }
+      }
+      if (!ok && lane == 0 && !*abortp) { atomicExch(p.status, I4T_ERR_MMA); *abortp = 1; }
+    } else if (warp == 2) {
+      int n = 0;
+      bool ok = true;
+      for (int w = first; w < n_items && ok; w += step) {
+        const I4TItem it = item_of(w);
+        if (it.n <= 0) continue;
+        // strips past the last one stay as they are in shared memory: their sums are not stored
+        const int s0 = (it.f0 + rank * (F / 2)) / I4_STRIP;
+        const int count = max(0, min(DUAL ? 4 : 8, p.strips - s0));
+        const unsigned bytes = (unsigned)(count * C::C_BYTES);
+        const size_t pitch = (size_t)p.strips * C::C_BYTES;
+        const unsigned char* from = reinterpret_cast<const unsigned char*>(p.data) +
+                                    ((size_t)it.e * (DUAL ? 2 : 1) * p.chunks + it.c0) * pitch +
+                                    (size_t)s0 * C::C_BYTES;
+        for (int c = it.c0; c < it.c1; ++c, ++n, from += pitch) {
+          const int s = n % C::C_RING;
+          ok = wait(&empty_c[s], (n / C::C_RING & 1) ^ 1);
+          if (!ok) break;
+          if (lane == 0) {
+            unsigned char* to = cs + s * 8 * C::C_BYTES;
+            mbar_expect_tx(&full_c[s], DUAL ? 2 * bytes : bytes);
+            if (bytes) {
+              i4t_copy(to, from, bytes, &full_c[s]);
+              if (DUAL) i4t_copy(to + 4 * C::C_BYTES, from + p.chunks * pitch, bytes, &full_c[s]);
             }
           }
           __syncwarp();
-          if (last) ++group;
         }
+      }
+      if (lane == 0) {
+        if (!ok && !*abortp) { atomicExch(p.status, I4T_ERR_CODES); *abortp = 1; }
+        for (int f = max(0, n - C::C_RING); f < n; ++f)
+          mbar_drain(&full_c[f % C::C_RING], f / C::C_RING & 1);
       }
     }
-    if (!ok && lane == 0 && !*abortp) { atomicExch(p.status, I4T_ERR_MMA); *abortp = 1; }
-  } else {
-    const int worker = warp - 2;
-    const int quarter = warp & 3, half = worker >> 2;  // lanes of tensor memory; every second 32 rows
+  } else if (warp >= 12) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    const int unpacker = warp - 12;          // strips 2 u and 2 u + 1
     const int g = lane >> 2, t = lane & 3;
     const bool odd = g & 1;
+    int n = 0;
     bool ok = true;
-    // strip s (0..7) of an item, as a block of the layout; strips past the last read the last
-    auto block_of = [&](const I4TItem& it, int s) {
-      const int strip = min(it.f0 / I4_STRIP + (DUAL ? (s & 3) : s), p.strips - 1);
-      const size_t matrix = DUAL ? 2 * (size_t)it.e + (s >> 2) : (size_t)it.e;
-      return (matrix * p.strips + strip) * p.chunks;
-    };
-    // -- the unpacking side: where the next chunk is, its codes and parameters in registers
-    int next_w = blockIdx.x, next_c = 0, tile = 0;
-    const unsigned *code_at = nullptr, *param_at = nullptr, *scale_at = nullptr;
-    uint4 code[2];
-    unsigned pa[NG], pb[NG], ps[NG];
-    auto words = [&](const unsigned* at, unsigned* v) {
+    for (int w = first; w < n_items && ok; w += step) {
+      const I4TItem it = item_of(w);
+      if (it.n <= 0) continue;
+      for (int c = it.c0; c < it.c1; ++c, ++n) {
+        const int sc = n % C::C_RING, sa = n % C::A_RING;
+        ok = wait(&full_c[sc], n / C::C_RING & 1);
+        if (!ok) break;
+        uint4 code[2][2];
+        unsigned pa[2][NG], pb[2][NG];
 #pragma unroll
-      for (int i = 0; i < NG; ++i) v[i] = __ldg(at + i);
-    };
-    auto fetch = [&]() {                     // the chunk at (next_w, next_c)
-      code[0] = __ldg(reinterpret_cast<const uint4*>(code_at));
-      code[1] = __ldg(reinterpret_cast<const uint4*>(code_at + I4_TILE_WORDS));
-      words(param_at, pa);
-      words(param_at + 8 * NG, pb);
-      words(scale_at, ps);
-    };
-    auto enter = [&]() {                     // the first chunk of the next item with rows
-      while (next_w < n_items) {
-        const I4TItem it = item_of(next_w);
-        if (it.n > 0) {
-          const size_t own = block_of(it, worker), row = block_of(it, 2 * quarter + (lane >> 4));
-          code_at = p.codes + own * I4_CHUNK_WORDS + lane * 4;
-          param_at = p.params + (own * I4_STRIP + g) * NG;
-          scale_at = p.params + (row * I4_STRIP + (lane & 15)) * NG;
-          next_c = 0;
-          fetch();
-          return;
-        }
-        next_w += gridDim.x;
-      }
-    };
-    float scale_next[NG];
-    auto unpack = [&]() {                    // the chunk in registers into two operand tiles
+        for (int u = 0; u < 2; ++u) {
+          // (DUAL: four gate strips were copied, then four up strips)
+          const unsigned* own = reinterpret_cast<const unsigned*>(
+              cs + (sc * 8 + (DUAL ? u * 4 + unpacker : unpacker * 2 + u)) * C::C_BYTES);
+          code[u][0] = *reinterpret_cast<const uint4*>(own + lane * 4);
+          code[u][1] = *reinterpret_cast<const uint4*>(own + I4_TILE_WORDS + lane * 4);
 #pragma unroll
-      for (int i = 0; i < NG; ++i) scale_next[i] = i4_scale(ps[i]);
-#pragma unroll
-      for (int h = 0; h < 2; ++h, ++tile) {
-        const int s = tile % C::A_RING;
-        ok = __all_sync(0xffffffffu, mbar_wait(&empty_a[s], ((tile / C::A_RING) & 1) ^ 1, abortp));
-        if (!ok) return;
-        unsigned char* at = as + s * I4T_A_BYTES + worker * 2048 + g * 128;
-#pragma unroll
-        for (int run = 0; run < 2; ++run) {
-          // lanes of odd rows take the two runs of eight k the other way round, so that the
-          // eight lanes of a store phase meet all banks
-          const bool second = (run == 1) != odd;
-          const unsigned w0 = second ? code[h].z : code[h].x;
-          const unsigned w1 = second ? code[h].w : code[h].y;
-          unsigned sa, sb;
-          if (GROUP == 32) {
-            sa = i4_sub(second ? pa[(2 * h + 1) % NG] : pa[2 * h % NG]);
-            sb = i4_sub(second ? pb[(2 * h + 1) % NG] : pb[2 * h % NG]);
-          } else {
-            sa = i4_sub(pa[GROUP == 64 ? h % NG : 0]);
-            sb = i4_sub(pb[GROUP == 64 ? h % NG : 0]);
+          for (int i = 0; i < NG; ++i) {
+            pa[u][i] = own[I4_CODE_WORDS + g * NG + i];
+            pb[u][i] = own[I4_CODE_WORDS + (g + 8) * NG + i];
           }
-          const int where = (((second ? 4 : 0) + t) ^ g) * 16;
-          *reinterpret_cast<uint4*>(at + where) = make_uint4(
-              i4_pair(w0, 0, sa), i4_pair(w0, 2, sa), i4_pair(w1, 0, sa), i4_pair(w1, 2, sa));
-          *reinterpret_cast<uint4*>(at + 1024 + where) = make_uint4(
-              i4_pair(w0, 1, sb), i4_pair(w0, 3, sb), i4_pair(w1, 1, sb), i4_pair(w1, 3, sb));
         }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty_c[sc]);
+        if (n >= C::A_RING) {
+          const int before = n - C::A_RING;
+          ok = wait(&done[before % I4T_DONE], before / I4T_DONE & 1);
+          if (!ok) break;
+        }
+        // the scales, by row and group, to the warps that add up
+        if (t == 0) {
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            unsigned short* to = scales + ((n % C::S_RING) * 128 + (unpacker * 2 + u) * 16 + g) * NG;
+            i4t_scales<NG>(to, pa[u]);
+            i4t_scales<NG>(to + 8 * NG, pb[u]);
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&full_s[n % C::S_RING]);
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            unsigned char* at = as + (sa * 2 + h) * I4T_TILE + (unpacker * 2 + u) * 2048 + g * 128;
+#pragma unroll
+            for (int run = 0; run < 2; ++run) {
+              // lanes of odd rows take the two runs of eight k the other way round, so that the
+              // eight lanes of a store phase meet all banks
+              const bool second = (run == 1) != odd;
+              const unsigned w0 = second ? code[u][h].z : code[u][h].x;
+              const unsigned w1 = second ? code[u][h].w : code[u][h].y;
+              unsigned sa2, sb2;
+              if (GROUP == 32) {
+                sa2 = i4_sub(second ? pa[u][(2 * h + 1) % NG] : pa[u][2 * h % NG]);
+                sb2 = i4_sub(second ? pb[u][(2 * h + 1) % NG] : pb[u][2 * h % NG]);
+              } else {
+                sa2 = i4_sub(pa[u][GROUP == 64 ? h % NG : 0]);
+                sb2 = i4_sub(pb[u][GROUP == 64 ? h % NG : 0]);
+              }
+              const int where = (((second ? 4 : 0) + t) ^ g) * 16;
+              *reinterpret_cast<uint4*>(at + where) =
+                  make_uint4(i4_pair(w0, 0, sa2), i4_pair(w0, 2, sa2), i4_pair(w1, 0, sa2),
+                             i4_pair(w1, 2, sa2));
+              *reinterpret_cast<uint4*>(at + 1024 + where) =
+                  make_uint4(i4_pair(w0, 1, sb2), i4_pair(w0, 3, sb2), i4_pair(w1, 1, sb2),
+                             i4_pair(w1, 3, sb2));
+            }
+          }
         fence_proxy_async();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&full_a[s]);
+        if (lane == 0) mbar_arrive(&full_a[sa]);
       }
-      if (++next_c < p.chunks) {
-        code_at += I4_CHUNK_WORDS;
-        param_at += I4_STRIP * NG;
-        scale_at += I4_STRIP * NG;
-        fetch();
-      } else {
-        next_w += gridDim.x;
-        enter();
-      }
-    };
-    // -- the summing side
-    int group = 0, handed = 0;
-    float sum[BT / 64][32];
-    enter();
-    if (next_w < n_items) unpack();
-    for (int w = blockIdx.x; w < n_items && ok; w += gridDim.x) {
+    }
+    if (!ok && lane == 0 && !*abortp) { atomicExch(p.status, I4T_ERR_UNPACK); *abortp = 1; }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+    const int quarter = warp & 3, half = (warp - 4) >> 2;  // lanes of tensor memory; every second 32 rows
+    const unsigned lanes = tmem_base + ((unsigned)(quarter * 32) << 16);
+    int n = 0, group = 0;
+    bool ok = true;
+    unsigned long long sum[BT / 64][16];     // pairs of rows
+    for (int w = first; w < n_items && ok; w += step) {
       const I4TItem it = item_of(w);
       if (it.n <= 0) continue;
 #pragma unroll
       for (int i = 0; i < BT / 64; ++i)
 #pragma unroll
-        for (int j = 0; j < 32; ++j) sum[i][j] = 0.f;
-      const unsigned lanes = tmem_base + ((unsigned)(quarter * 32) << 16);
-      for (int c = 0; c < p.chunks && ok; ++c) {
-        float scale[NG];
-#pragma unroll
-        for (int i = 0; i < NG; ++i) scale[i] = scale_next[i];
-        if (next_w < n_items) unpack();
+        for (int j = 0; j < 16; ++j) sum[i][j] = 0;
+      for (int c = it.c0; c < it.c1 && ok; ++c, ++n) {
+        ok = wait(&full_s[n % C::S_RING], n / C::S_RING & 1);
         if (!ok) break;
+        unsigned long long scale[NG];
 #pragma unroll
-        for (int n = 0; n < NG; ++n, ++group) {
+        for (int q = 0; q < NG; ++q) {
+          const float v = i4_scale(scales[((n % C::S_RING) * 128 + quarter * 32 + lane) * NG + q]);
+          scale[q] = i4t_pack(v, v);
+        }
+#pragma unroll
+        for (int q = 0; q < NG; ++q, ++group) {
           const int buf = group & 1;
-          ok = __all_sync(0xffffffffu, mbar_wait(&acc_full[buf], (group >> 1) & 1, abortp));
+          ok = NG == 1 ? wait(&done[n % I4T_DONE], n / I4T_DONE & 1)
+                       : wait(&acc_full[buf], group >> 1 & 1);
           if (!ok) break;
           tc_fence_after();
 #pragma unroll
@@ -361,7 +514,8 @@ int4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const I4TArgs p) {
               float v[32];
               tc_ld32(lanes + buf * BT + col, v);
 #pragma unroll
-              for (int j = 0; j < 32; ++j) sum[i][j] = fmaf(scale[n], v[j], sum[i][j]);
+              for (int j = 0; j < 16; ++j)
+                i4t_fma2(sum[i][j], scale[q], i4t_pack(v[2 * j], v[2 * j + 1]));
             }
           }
           tc_fence_before();
@@ -371,116 +525,127 @@ int4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const I4TArgs p) {
       }
       if (!ok) break;
       // -- a lane holds one weight row for 32 rows at a time: 64- or 128-byte stores of a warp
-      if (DUAL) {
-        // the warps of the up rows (quarters 2, 3) hand their sums to those of the gate rows
-        const int pair = (quarter & 1) + 2 * half;
-        float* mine = exchange + pair * (32 * 33);
-        const int f = it.f0 + (quarter & 1) * 32 + lane;
+      const int f_own = it.f0 + rank * (F / 2);
+      if (p.splits > 1) {
+        // sums of a run of K: the halves' columns beside each other
+        const int f = DUAL ? f_own + quarter * 16 + (lane & 15) : f_own + quarter * 32 + lane;
+        const size_t width = DUAL ? 2 * (size_t)p.N : (size_t)p.N;
+        float* o = p.part + ((size_t)it.z * p.rows + it.m0) * width +
+                   (DUAL && lane >= 16 ? p.N : 0) + f;
 #pragma unroll
         for (int i = 0; i < BT / 64; ++i) {
           const int col = 64 * i + 32 * half;
-          if (col >= it.n) continue;
-          if (quarter >= 2) {
-            ok = __all_sync(0xffffffffu, mbar_wait(&ex_empty[pair], (handed & 1) ^ 1, abortp));
-            if (!ok) break;
+          const int n_here = f < p.N ? it.n - col : 0;
 #pragma unroll
-            for (int j = 0; j < 32; ++j) mine[j * 33 + lane] = sum[i][j];
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&ex_full[pair]);
-            ++handed;
-          } else {
-            ok = __all_sync(0xffffffffu, mbar_wait(&ex_full[pair], handed & 1, abortp));
-            if (!ok) break;
-            ++handed;
-            const float rs = p.row_scale && col + lane < it.n ? p.row_scale[it.m0 + col + lane] : 1.f;
-            float y[32];
+          for (int j = 0; j < 16; ++j) {
+            float a, b;
+            i4t_unpack(sum[i][j], a, b);
+            if (2 * j < n_here) o[(size_t)(col + 2 * j) * width] = a;
+            if (2 * j + 1 < n_here) o[(size_t)(col + 2 * j + 1) * width] = b;
+          }
+        }
+      } else if (DUAL) {
+        // of two neighbouring rows the lanes with the gate's sums take the first, those with the
+        // up sums the second: each gets the other sum of its row
+        const bool up = lane >= 16;
+        const int f = f_own + quarter * 16 + (lane & 15);
 #pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              const float s = __shfl_sync(0xffffffffu, rs, j);
-              const float a = sum[i][j] * s, u = mine[j * 33 + lane] * s;
-              y[j] = p.wide ? a / (1.0f + expf(-a)) * u : __fdividef(a, 1.0f + __expf(-a)) * u;
+        for (int i = 0; i < BT / 64; ++i) {
+          const int col = 64 * i + 32 * half + (up ? 1 : 0);
+          if (64 * i + 32 * half >= it.n) continue;
+          const int n_here = f < p.N ? it.n - col : 0;
+          const size_t at = (size_t)(it.m0 + col) * p.N + f;
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            float first_row, second_row;
+            i4t_unpack(sum[i][j], first_row, second_row);
+            const float got = __shfl_xor_sync(0xffffffffu, up ? first_row : second_row, 16);
+            float a = up ? got : first_row, u = up ? second_row : got;
+            if (p.row_scale) {
+              const float s = 2 * j < n_here ? p.row_scale[it.m0 + col + 2 * j] : 0.f;
+              a *= s;
+              u *= s;
             }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&ex_empty[pair]);
-            const int n_here = f < p.N ? it.n - col : 0;
-            const size_t at = (size_t)(it.m0 + col) * p.N + f;
             if (p.wide) {
-              float* o = (float*)p.out + at;
-#pragma unroll
-              for (int j = 0; j < 32; ++j)
-                if (j < n_here) o[(size_t)j * p.N] = y[j];
+              const float y = i4t_silu_wide(a, u);
+              if (2 * j < n_here) ((float*)p.out)[at + (size_t)(2 * j) * p.N] = y;
             } else {
-              bf16* o = (bf16*)p.out + at;
-#pragma unroll
-              for (int j = 0; j < 32; ++j)
-                if (j < n_here) o[(size_t)j * p.N] = __float2bfloat16_rn(y[j]);
+              const float y = __fdividef(a, 1.0f + __expf(-a)) * u;
+              if (2 * j < n_here)
+                ((bf16*)p.out)[at + (size_t)(2 * j) * p.N] = __float2bfloat16_rn(y);
             }
           }
         }
       } else {
-        const int f = it.f0 + quarter * 32 + lane;
+        const int f = f_own + quarter * 32 + lane;
 #pragma unroll
-        for (int i = 0; i < BT / 64; ++i) {
-          const int col = 64 * i + 32 * half;
+        for (int i = 0; i < BT / 32; ++i) {            // sixteen rows at a time
+          const int col = 64 * (i >> 1) + 32 * half + 16 * (i & 1);
           if (col >= it.n) continue;
-          const int n_here = f < p.N ? it.n - col : 0;
-          const size_t at = (size_t)(it.m0 + col) * p.N + f;
-          if (p.plain) {
+          float v[16];
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
-              sum[i][j] = p.wide ? ix_act<float>(sum[i][j], p.plain) : ix_act<bf16>(sum[i][j], p.plain);
-          }
-          if (p.wide) {
-            float* o = (float*)p.out + at;
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (j < n_here) o[(size_t)j * p.N] = sum[i][j];
-          } else {
-            bf16* o = (bf16*)p.out + at;
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (j < n_here) o[(size_t)j * p.N] = __float2bfloat16_rn(sum[i][j]);
-          }
+          for (int j = 0; j < 8; ++j) i4t_unpack(sum[i >> 1][8 * (i & 1) + j], v[2 * j], v[2 * j + 1]);
+          i4t_store<16>(p, v, f < p.N ? it.n - col : 0, (size_t)(it.m0 + col) * p.N + f);
         }
       }
     }
-    if (!ok && lane == 0 && !*abortp) { atomicExch(p.status, I4T_ERR_WORK); *abortp = 1; }
+    if (!ok && lane == 0 && !*abortp) { atomicExch(p.status, I4T_ERR_SUM); *abortp = 1; }
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 1) tc_dealloc<false>(tmem_base, C::TMEM_COLS);
+  // neither block ends while the other can still reach its barriers, tiles or accumulators
+  tc_cluster_sync();
+  if (warp == 1) tc_dealloc<true>(tmem_base, C::TMEM_COLS);
+}
+
+// The runs' sums in ascending order, and what follows them.
+template <bool DUAL>
+__global__ void __launch_bounds__(256)
+int4_join_kernel(const I4TArgs p) {
+  const int f = blockIdx.x * 256 + threadIdx.x;
+  const size_t r = blockIdx.y;
+  if (f >= p.N) return;
+  const size_t width = DUAL ? 2 * (size_t)p.N : (size_t)p.N, plane = (size_t)p.rows * width;
+  const float* from = p.part + r * width + f;
+  float a = 0.f, u = 0.f;
+  for (int z = 0; z < p.splits; ++z, from += plane) {
+    a += from[0];
+    if (DUAL) u += from[p.N];
+  }
+  if (DUAL) {
+    if (p.row_scale) {
+      a *= p.row_scale[r];
+      u *= p.row_scale[r];
+    }
+    a = p.wide ? a / (1.0f + expf(-a)) * u : __fdividef(a, 1.0f + __expf(-a)) * u;
+  } else if (p.plain) {
+    a = p.wide ? ix_act<float>(a, p.plain) : ix_act<bf16>(a, p.plain);
+  }
+  if (p.wide) ((float*)p.out)[r * p.N + f] = a;
+  else ((bf16*)p.out)[r * p.N + f] = __float2bfloat16_rn(a);
 }
 
 template <int TERMS, bool DUAL, int BT, int GROUP>
-static int i4t_launch(const void* x, int x_rows, int Kp, I4TArgs p, int sms, cudaStream_t stream) {
+static int i4t_launch(const void* x, int Kp, const I4TArgs& p, int sms, cudaStream_t stream) {
   typedef I4TCfg<TERMS, DUAL, BT, GROUP> C;
   CUtensorMap map;
-  const int rc = ix_tensor_map_bf16_2d(&map, x, (long long)TERMS * x_rows, Kp, 64, I4T_BOX);
+  const int rc = ix_tensor_map_bf16_2d(&map, x, (long long)TERMS * p.rows, Kp, 64, C::BOX);
   if (rc != IX_OK) return rc;
   const long long tiles = p.offsets ? (p.rows + BT - 1) / BT + (long long)p.E
                                     : (p.rows + p.tile_rows - 1) / p.tile_rows;
-  const long long items = tiles * ((p.N + C::F - 1) / C::F);
+  const long long items = tiles * ((p.N + C::F - 1) / C::F) * p.splits;
   if (items > 0x7fffffffLL) return IX_ERR_SIZE;
   auto kern = int4_tc_kernel<TERMS, DUAL, BT, GROUP>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
   if (e != cudaSuccess) return (int)e;
-  kern<<<(int)(items < sms ? items : sms), I4T_THREADS, C::SMEM, stream>>>(map, p);
+  const int pairs = sms / 2;
+  kern<<<2 * (int)(items < pairs ? items : pairs), I4T_THREADS, C::SMEM, stream>>>(map, p);
+  if (p.splits > 1)
+    int4_join_kernel<DUAL><<<dim3((p.N + 255) / 256, p.rows), 256, 0, stream>>>(p);
   return ix_launch_status();
 }
 
-// x: [rows, Kp] bf16, or [3, rows, Kp] terms of fp32 rows; Kp a multiple of 8 that ends in the last
-// chunk.  out: [rows, N] fp32 (wide) or bf16.  offsets == null: one matrix.  status: one int, zero
-// before the first call.
-IX_API int ix_int4_tc(const void* x, int terms, const int* offsets, const void* codes,
-                      const void* params, void* out, int wide, int dual, int rows, int N, int Kp,
-                      int E, int group, const float* row_scale, int plain, int* status,
-                      cudaStream_t stream) {
-  if ((row_scale && !dual) || (plain && dual)) return IX_ERR_UNSUPPORTED;
-  if (rows <= 0) return IX_OK;
-  if (N <= 0 || Kp <= 0 || E <= 0 || status == nullptr) return IX_ERR_SIZE;
-  if (Kp % 8 != 0 || E > I4T_MAX_EXPERTS || (!offsets && E != 1)) return IX_ERR_UNSUPPORTED;
-  if ((uintptr_t)x & 15) return IX_ERR_ALIGN;
-  if (3LL * rows > 0x7fffffffLL) return IX_ERR_SIZE;
+static int i4t_sms() {
   static int sms = 0;
   if (sms == 0) {
     int dev = 0;
@@ -488,44 +653,91 @@ IX_API int ix_int4_tc(const void* x, int terms, const int* offsets, const void* 
     if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms <= 0)
       sms = 148;
   }
-  I4TArgs p = {offsets, (const unsigned*)codes, (const unsigned*)params, out, wide, row_scale, plain,
-               rows, N, (int)i4_strips(N), (int)i4_chunks(Kp), E, 0, rows, status};
-  const int f = dual ? 64 : 128;
+  return sms;
+}
+
+// How a call is cut: rows of a tile (one matrix) and runs of K.
+struct I4TPlan {
+  int tile_rows, splits;
   bool large;
-  if (offsets) {
-    large = 1.15 * rows / E > 128.0;      // the mean rows of an expert, and some for imbalance
-  } else {
-    large = rows > 128;
-    const int most = large && terms == 1 ? 256 : 128;
-    // as many tiles as give the least work: waves of blocks times the rows of a tile (and some
-    // that a tile costs whatever its rows)
-    const int f_tiles = (N + f - 1) / f;
-    long long best = -1;
-    for (int cuts = (rows + most - 1) / most; cuts <= (rows + most - 1) / most + 8; ++cuts) {
-      const int per = ((rows + cuts - 1) / cuts + 15) & ~15;
-      const long long items = (long long)((rows + per - 1) / per) * f_tiles;
-      const long long cost = (items + sms - 1) / sms * (per + 32);
-      if (best < 0 || cost < best) {
-        best = cost;
-        p.tile_rows = per;
-      }
-      if (per <= 16) break;
-    }
-    large = p.tile_rows > 128;
+};
+
+static I4TPlan i4t_plan(int rows, int N, int Kp, int E, bool grouped, bool dual, int terms) {
+  const int pairs = i4t_sms() / 2, f = dual ? 128 : 256, chunks = (int)i4_chunks(Kp);
+  const long long f_tiles = (N + f - 1) / f;
+  I4TPlan plan = {0, 1, false};
+  double best = -1;
+  if (grouped) {
+    // the mean rows of an expert, and some for imbalance
+    plan.large = terms == 1 && 1.15 * rows / E > 128.0;
+    plan.tile_rows = plan.large ? 256 : 128;
+    const long long tiles = (rows < E ? rows : E) * f_tiles;
+    while (rows <= 4096 && plan.splits < 16 && tiles * plan.splits * 2 <= pairs && chunks / (plan.splits * 2) >= 2)
+      plan.splits *= 2;
+    return plan;
   }
-#define I4T_BT(T, D, B)                                                               \
-  do {                                                                                \
-    if (group == 128) return i4t_launch<T, D, B, 128>(x, rows, Kp, p, sms, stream);   \
-    if (group == 64) return i4t_launch<T, D, B, 64>(x, rows, Kp, p, sms, stream);     \
-    if (group == 32) return i4t_launch<T, D, B, 32>(x, rows, Kp, p, sms, stream);     \
-    return IX_ERR_UNSUPPORTED;                                                        \
+  const int most = rows > 128 && terms == 1 ? 256 : 128;
+  const int cuts0 = (rows + most - 1) / most;
+  for (int cuts = cuts0; cuts <= cuts0 + 8; ++cuts) {
+    const int per = ((rows + cuts - 1) / cuts + 31) & ~31;
+    for (int splits = 1; splits <= (rows > 4096 ? 1 : 16) && splits <= chunks; ++splits) {
+      const int run = (chunks + splits - 1) / splits;
+      if ((long long)run * (splits - 1) >= chunks) continue;      // an empty last run
+      const long long items = (long long)((rows + per - 1) / per) * f_tiles * splits;
+      const double us = (double)((items + pairs - 1) / pairs) * (run * (0.25 + 0.0015 * terms * per) + 1.5) +
+                        (splits > 1 ? 2.0 + splits * (double)rows * N * (dual ? 2 : 1) * 1.6e-6 : 0.0);
+      if (best < 0 || us < 0.98 * best) {
+        best = us;
+        plan.tile_rows = per;
+        plan.splits = splits;
+      }
+    }
+    if (per <= 32) break;
+  }
+  plan.large = plan.tile_rows > 128;
+  return plan;
+}
+
+// fp32 entries of scratch that a call of these sizes wants (0: none)
+IX_API long long ix_int4_tc_scratch(int rows, int N, int Kp, int E, int grouped, int dual, int terms) {
+  if (rows <= 0 || N <= 0 || Kp <= 0 || E <= 0) return 0;
+  const I4TPlan plan = i4t_plan(rows, N, Kp, E, grouped != 0, dual != 0, terms);
+  return plan.splits > 1 ? (long long)plan.splits * rows * N * (dual ? 2 : 1) : 0;
+}
+
+// x: [rows, Kp] bf16, or [3, rows, Kp] terms of fp32 rows; Kp a multiple of 8 that ends in the last
+// chunk.  out: [rows, N] fp32 (wide) or bf16.  offsets == null: one matrix.  part: scratch of the size
+// that ix_int4_tc_scratch names, or null where it names none.  status: one int, zero before the first
+// call.
+IX_API int ix_int4_tc(const void* x, int terms, const int* offsets, const void* data, void* out,
+                      float* part, int wide, int dual, int rows, int N, int Kp, int E, int group,
+                      const float* row_scale, int plain, int* status, cudaStream_t stream) {
+  if ((row_scale && !dual) || (plain && dual)) return IX_ERR_UNSUPPORTED;
+  if (rows <= 0) return IX_OK;
+  if (N <= 0 || Kp <= 0 || E <= 0 || status == nullptr) return IX_ERR_SIZE;
+  if (Kp % 8 != 0 || E > I4T_MAX_EXPERTS || (!offsets && E != 1)) return IX_ERR_UNSUPPORTED;
+  if (((uintptr_t)x | (uintptr_t)data) & 15) return IX_ERR_ALIGN;
+  if (3LL * rows > 0x7fffffffLL || N > 0x3fffff00) return IX_ERR_SIZE;
+  const I4TPlan plan = i4t_plan(rows, N, Kp, E, offsets != nullptr, dual != 0, terms);
+  if (plan.splits > 1 && (part == nullptr || rows > 65535)) return IX_ERR_SIZE;
+  const int chunks = (int)i4_chunks(Kp);
+  const I4TArgs p = {offsets, (const unsigned*)data, out, part, wide, row_scale, plain, rows, N,
+                     (int)i4_strips(N), chunks, E, plan.tile_rows, plan.splits,
+                     (chunks + plan.splits - 1) / plan.splits, rows, status};
+  const int sms = i4t_sms();
+#define I4T_BT(T, D, B)                                                       \
+  do {                                                                        \
+    if (group == 128) return i4t_launch<T, D, B, 128>(x, Kp, p, sms, stream); \
+    if (group == 64) return i4t_launch<T, D, B, 64>(x, Kp, p, sms, stream);   \
+    if (group == 32) return i4t_launch<T, D, B, 32>(x, Kp, p, sms, stream);   \
+    return IX_ERR_UNSUPPORTED;                                                \
   } while (0)
   if (terms == 1) {
     if (dual) {
-      if (large) I4T_BT(1, true, 256);
+      if (plan.large) I4T_BT(1, true, 256);
       I4T_BT(1, true, 128);
     }
-    if (large) I4T_BT(1, false, 256);
+    if (plan.large) I4T_BT(1, false, 256);
     I4T_BT(1, false, 128);
   }
   if (terms == 3) {

@@ -43,11 +43,14 @@ struct I4Place {
 __device__ __forceinline__ bool i4_place(I4Place& p, long long matrices, int strips, int chunks) {
   const long long w = (long long)blockIdx.x * I4_WARPS + (threadIdx.x >> 5);
   if (w >= matrices * strips * chunks) return false;
-  p.chunk = (int)(w % chunks);
+  p.chunk = (int)(w % chunks);               // (neighbouring warps read a row's neighbouring k)
   const long long s = w / chunks;
   p.strip = (int)(s % strips);
   p.m = s / strips;
   return true;
+}
+__device__ __forceinline__ size_t i4_block(const I4Place& p, int strips, int chunks) {
+  return ((size_t)p.m * chunks + p.chunk) * strips + p.strip;
 }
 
 // The 32 entries of a row that a lane of `t` holds of a chunk, from `src` (the row, or null: zeros).
@@ -105,15 +108,15 @@ __device__ __forceinline__ void i4_store_words(unsigned* dst, int lane, const un
 
 template <typename T, int GROUP>
 __global__ void __launch_bounds__(I4_WARPS * 32)
-i4_quantize_kernel(const T* __restrict__ w, unsigned* __restrict__ codes,
-                   unsigned* __restrict__ params, long long matrices, int rows, int K, int strips,
+i4_quantize_kernel(const T* __restrict__ w, unsigned* __restrict__ data,
+                   long long matrices, int rows, int K, int strips,
                    int chunks, int vec) {
   constexpr int PER = GROUP / 32, NG = 4 / PER;    // blocks of 32 a group, groups a chunk
   I4Place p;
   if (!i4_place(p, matrices, strips, chunks)) return;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int k0 = p.chunk * I4_CHUNK_K;
-  const size_t block = ((size_t)p.m * strips + p.strip) * chunks + p.chunk;
+  const size_t block = i4_block(p, strips, chunks) * i4_block_words(GROUP);
   unsigned char code[2][32];
 #pragma unroll
   for (int side = 0; side < 2; ++side) {
@@ -148,25 +151,26 @@ i4_quantize_kernel(const T* __restrict__ w, unsigned* __restrict__ codes,
         const float c = fminf(fmaxf(i4_rint_ratio(v[at], s) + zero, 0.f), 15.f);
         code[side][at] = some ? (unsigned char)(int)c : 0;
       }
-      if (t == 0) params[(block * I4_STRIP + g + side * 8) * NG + n] = i4_param(scale, (int)zero);
+      if (t == 0)
+        data[block + I4_CODE_WORDS + (g + side * 8) * NG + n] = i4_param(scale, (int)zero);
     }
   }
-  i4_store_words(codes + block * I4_CHUNK_WORDS, lane, code[0], code[1]);
+  i4_store_words(data + block, lane, code[0], code[1]);
 }
 
 // Codes, scales and zero points of a caller's own into the layout.
 template <int GROUP>
 __global__ void __launch_bounds__(I4_WARPS * 32)
 i4_pack_kernel(const unsigned char* __restrict__ in, const bf16* __restrict__ scales,
-               const unsigned char* __restrict__ zeros, unsigned* __restrict__ codes,
-               unsigned* __restrict__ params, long long matrices, int rows, int K, int strips,
+               const unsigned char* __restrict__ zeros, unsigned* __restrict__ data,
+               long long matrices, int rows, int K, int strips,
                int chunks, int vec) {
   constexpr int PER = GROUP / 32, NG = 4 / PER;
   I4Place p;
   if (!i4_place(p, matrices, strips, chunks)) return;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int k0 = p.chunk * I4_CHUNK_K, groups = (K + GROUP - 1) / GROUP;
-  const size_t block = ((size_t)p.m * strips + p.strip) * chunks + p.chunk;
+  const size_t block = i4_block(p, strips, chunks) * i4_block_words(GROUP);
   unsigned char code[2][32];
 #pragma unroll
   for (int side = 0; side < 2; ++side) {
@@ -194,17 +198,17 @@ i4_pack_kernel(const unsigned char* __restrict__ in, const bf16* __restrict__ sc
             code[side][at + i] = there && k + i < K ? in[r * K + k + i] & 15 : zero;
         }
       }
-      if (t == 0) params[(block * I4_STRIP + g + side * 8) * NG + n] = i4_param(scale, zero);
+      if (t == 0)
+        data[block + I4_CODE_WORDS + (g + side * 8) * NG + n] = i4_param(scale, zero);
     }
   }
-  i4_store_words(codes + block * I4_CHUNK_WORDS, lane, code[0], code[1]);
+  i4_store_words(data + block, lane, code[0], code[1]);
 }
 
 // The layout back to codes, scales and zero points.
 template <int GROUP>
 __global__ void __launch_bounds__(I4_WARPS * 32)
-i4_unpack_kernel(const unsigned* __restrict__ codes, const unsigned* __restrict__ params,
-                 unsigned char* __restrict__ out, bf16* __restrict__ scales,
+i4_unpack_kernel(const unsigned* __restrict__ data, unsigned char* __restrict__ out, bf16* __restrict__ scales,
                  unsigned char* __restrict__ zeros, long long matrices, int rows, int K, int strips,
                  int chunks, int vec) {
   constexpr int NG = 128 / GROUP;
@@ -212,11 +216,11 @@ i4_unpack_kernel(const unsigned* __restrict__ codes, const unsigned* __restrict_
   if (!i4_place(p, matrices, strips, chunks)) return;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int k0 = p.chunk * I4_CHUNK_K, groups = (K + GROUP - 1) / GROUP;
-  const size_t block = ((size_t)p.m * strips + p.strip) * chunks + p.chunk;
+  const size_t block = i4_block(p, strips, chunks) * i4_block_words(GROUP);
   uint4 w[2];
 #pragma unroll
   for (int tile = 0; tile < 2; ++tile)
-    w[tile] = *reinterpret_cast<const uint4*>(codes + block * I4_CHUNK_WORDS +
+    w[tile] = *reinterpret_cast<const uint4*>(data + block +
                                               tile * I4_TILE_WORDS + lane * 4);
 #pragma unroll
   for (int side = 0; side < 2; ++side) {
@@ -245,7 +249,7 @@ i4_unpack_kernel(const unsigned* __restrict__ codes, const unsigned* __restrict_
     for (int n = t; n < NG; n += 4) {
       const int group = p.chunk * NG + n;
       if (group >= groups) continue;
-      const unsigned param = params[(block * I4_STRIP + g + side * 8) * NG + n];
+      const unsigned param = data[block + I4_CODE_WORDS + (g + side * 8) * NG + n];
       scales[r * groups + group] = __ushort_as_bfloat16((unsigned short)param);
       zeros[r * groups + group] = (unsigned char)((param >> 16) - 0x4300u);
     }
@@ -270,10 +274,9 @@ static int i4_grid(long long matrices, int rows, int K, int& strips, int& chunks
     else return IX_ERR_UNSUPPORTED;                                            \
   } while (0)
 
-// w: [matrices, rows, K] fp32 or bf16.  codes: [matrices, strips, chunks, 256] words; params:
-// [matrices, strips, chunks, 16, 128 / group] words.
-IX_API int ix_int4_quantize(const void* w, int dtype, void* codes, void* params,
-                            long long matrices, int rows, int K, int group, cudaStream_t stream) {
+// w: [matrices, rows, K] fp32 or bf16.  data: [matrices, chunks, strips, words of a block].
+IX_API int ix_int4_quantize(const void* w, int dtype, void* data, long long matrices, int rows, int K,
+                            int group, cudaStream_t stream) {
   int strips, chunks;
   unsigned grid;
   const int rc = i4_grid(matrices, rows, K, strips, chunks, grid);
@@ -281,15 +284,15 @@ IX_API int ix_int4_quantize(const void* w, int dtype, void* codes, void* params,
   const int vec = K % 8 == 0 && ((uintptr_t)w & 15) == 0;
   IX_DISPATCH_DTYPE(dtype, T, {
     I4_GROUPS(G, i4_quantize_kernel<T, G><<<grid, I4_WARPS * 32, 0, stream>>>(
-                     (const T*)w, (unsigned*)codes, (unsigned*)params, matrices, rows, K, strips,
+                     (const T*)w, (unsigned*)data, matrices, rows, K, strips,
                      chunks, vec));
   });
   return ix_launch_status();
 }
 
 // in: [matrices, rows, K] bytes; scales bf16 and zeros bytes: [matrices, rows, ceil(K / group)].
-IX_API int ix_int4_pack(const void* in, const void* scales, const void* zeros, void* codes,
-                        void* params, long long matrices, int rows, int K, int group,
+IX_API int ix_int4_pack(const void* in, const void* scales, const void* zeros, void* data,
+                        long long matrices, int rows, int K, int group,
                         cudaStream_t stream) {
   int strips, chunks;
   unsigned grid;
@@ -298,11 +301,11 @@ IX_API int ix_int4_pack(const void* in, const void* scales, const void* zeros, v
   const int vec = K % 8 == 0 && ((uintptr_t)in & 7) == 0;
   I4_GROUPS(G, i4_pack_kernel<G><<<grid, I4_WARPS * 32, 0, stream>>>(
                    (const unsigned char*)in, (const bf16*)scales, (const unsigned char*)zeros,
-                   (unsigned*)codes, (unsigned*)params, matrices, rows, K, strips, chunks, vec));
+                   (unsigned*)data, matrices, rows, K, strips, chunks, vec));
   return ix_launch_status();
 }
 
-IX_API int ix_int4_unpack(const void* codes, const void* params, void* out, void* scales,
+IX_API int ix_int4_unpack(const void* data, void* out, void* scales,
                           void* zeros, long long matrices, int rows, int K, int group,
                           cudaStream_t stream) {
   int strips, chunks;
@@ -311,8 +314,8 @@ IX_API int ix_int4_unpack(const void* codes, const void* params, void* out, void
   if (rc != IX_OK) return rc;
   const int vec = K % 8 == 0 && ((uintptr_t)out & 7) == 0;
   I4_GROUPS(G, i4_unpack_kernel<G><<<grid, I4_WARPS * 32, 0, stream>>>(
-                   (const unsigned*)codes, (const unsigned*)params, (unsigned char*)out,
-                   (bf16*)scales, (unsigned char*)zeros, matrices, rows, K, strips, chunks, vec));
+                   (const unsigned*)data, (unsigned char*)out, (bf16*)scales,
+                   (unsigned char*)zeros, matrices, rows, K, strips, chunks, vec));
   return ix_launch_status();
 }
 

@@ -1342,6 +1342,7 @@ _STATUS_ROLES = {
     34: "widened_attention: shared memory not on a 1024-byte mark;",
     41: "gemm_fp32_tc: a splitting warp", 42: "gemm_fp32_tc: the MMA issuer",
     51: "int4_tc: the copying warp", 52: "int4_tc: the MMA issuer", 53: "int4_tc: an unpacking warp",
+    54: "int4_tc: the warp that copies codes", 55: "int4_tc: a warp that adds up",
 }
 
 
@@ -1514,20 +1515,18 @@ class Int4Weight:
     a code in 0..15 that stands for ``scale * (code - zero)``.  Made by ``quantize_int4`` or
     ``pack_int4``; ``linear`` and the gated and grouped products take it where they take a
     matrix.  ``halves`` is 2 where the rows are a gate matrix and then an up matrix of the same
-    size, which the gated products want, and 1 otherwise.  ``codes`` and ``params`` are int32
-    tensors in the kernels' own layout."""
+    size, which the gated products want, and 1 otherwise.  ``data`` is an int32 tensor in the
+    kernels' own layout."""
 
-    __slots__ = ("shape", "halves", "group_size", "codes", "params")
+    __slots__ = ("shape", "halves", "group_size", "data")
 
-    def __init__(self, shape, halves: int, group_size: int, codes: torch.Tensor,
-                 params: torch.Tensor):
+    def __init__(self, shape, halves: int, group_size: int, data: torch.Tensor):
         self.shape = torch.Size(shape)
-        self.halves, self.group_size = halves, group_size
-        self.codes, self.params = codes, params
+        self.halves, self.group_size, self.data = halves, group_size, data
 
     @property
     def device(self):
-        return self.codes.device
+        return self.data.device
 
     @property
     def experts(self) -> int:
@@ -1540,7 +1539,7 @@ class Int4Weight:
 
     @property
     def nbytes(self) -> int:
-        return self.codes.nbytes + self.params.nbytes
+        return self.data.nbytes
 
     def numel(self) -> int:
         return self.shape.numel()
@@ -1561,10 +1560,9 @@ def _int4_empty(what: str, shape, group_size: int, halves: int, device) -> Int4W
     matrices = (shape[0] if len(shape) == 3 else 1) * halves
     strips = -(-(shape[-2] // halves) // INT4_LAYOUT_ROWS)
     chunks = -(-shape[-1] // INT4_LAYOUT_K)
-    codes = torch.empty((matrices, strips, chunks, 256), dtype=torch.int32, device=device)
-    params = torch.empty((matrices, strips, chunks, 16, 128 // group_size), dtype=torch.int32,
-                         device=device)
-    return Int4Weight(shape, halves, group_size, codes, params)
+    data = torch.empty((matrices, chunks, strips, 256 + 16 * (128 // group_size)),
+                       dtype=torch.int32, device=device)
+    return Int4Weight(shape, halves, group_size, data)
 
 
 def _on_current_device(what: str, *tensors):
@@ -1585,7 +1583,7 @@ def quantize_int4(w: torch.Tensor, group_size: int = 128, halves: int = 1) -> In
     code = _dtype_code(w)
     _on_current_device("quantize_int4", w)
     q = _int4_empty("quantize_int4", w.shape, group_size, halves, w.device)
-    _check(_lib().ix_int4_quantize(_ptr(w), code, _ptr(q.codes), _ptr(q.params),
+    _check(_lib().ix_int4_quantize(_ptr(w), code, _ptr(q.data),
                                    ctypes.c_longlong(q.experts * halves), q.cols, w.shape[-1],
                                    group_size, _stream()), "quantize_int4")
     _count()
@@ -1608,8 +1606,8 @@ def pack_int4(codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor,
                           f"{list(scales.shape)} and {list(zeros.shape)}")
     if int(torch.maximum(codes.max(), zeros.max())) > 15:
         raise KernelError("pack_int4: codes and zeros must lie in 0..15")
-    _check(_lib().ix_int4_pack(_ptr(codes), _ptr(scales), _ptr(zeros), _ptr(q.codes),
-                               _ptr(q.params), ctypes.c_longlong(q.experts * halves), q.cols,
+    _check(_lib().ix_int4_pack(_ptr(codes), _ptr(scales), _ptr(zeros), _ptr(q.data),
+                               ctypes.c_longlong(q.experts * halves), q.cols,
                                codes.shape[-1], group_size, _stream()), "pack_int4")
     _count()
     return q
@@ -1619,12 +1617,12 @@ def unpack_int4(w: Int4Weight):
     """(codes, scales, zeros) of an ``Int4Weight``, as ``pack_int4`` takes them."""
     if not isinstance(w, Int4Weight):
         raise KernelError(f"unpack_int4: expected an Int4Weight, got {type(w).__name__}")
-    _on_current_device("unpack_int4", w.codes)
+    _on_current_device("unpack_int4", w.data)
     groups = (*w.shape[:-1], -(-w.shape[-1] // w.group_size))
     codes = torch.empty(w.shape, dtype=torch.uint8, device=w.device)
     scales = torch.empty(groups, dtype=torch.bfloat16, device=w.device)
     zeros = torch.empty(groups, dtype=torch.uint8, device=w.device)
-    _check(_lib().ix_int4_unpack(_ptr(w.codes), _ptr(w.params), _ptr(codes), _ptr(scales),
+    _check(_lib().ix_int4_unpack(_ptr(w.data), _ptr(codes), _ptr(scales),
                                  _ptr(zeros), ctypes.c_longlong(w.experts * w.halves), w.cols,
                                  w.shape[-1], w.group_size, _stream()), "unpack_int4")
     _count()
@@ -1636,7 +1634,7 @@ def _int4_operands(what: str, x: torch.Tensor, w: Int4Weight, halves: int, dims:
     """The checks that every product with an ``Int4Weight`` makes; the code of x's type."""
     _chk("x", x)
     code = _dtype_code(x)
-    _on_current_device(what, x, w.codes, *others)
+    _on_current_device(what, x, w.data, *others)
     if x.dim() != 2 or len(w.shape) != dims or x.shape[1] != w.shape[-1]:
         raise KernelError(f"{what}: activations {list(x.shape)} against weights "
                           f"{list(w.shape)}")
@@ -1666,7 +1664,7 @@ def _int4_stream(what, x, rows, offsets, w, num_rows, out_dtype, rows_per_pass, 
         offsets_settled = False            # one launch more in front of this one
     out = torch.empty((num_rows, w.cols), dtype=out_dtype, device=x.device)
     _check(_lib().ix_int4_stream(
-        _ptr(x), _dtype_code(x), _ptr(rows), _ptr(offsets), _ptr(w.codes), _ptr(w.params),
+        _ptr(x), _dtype_code(x), _ptr(rows), _ptr(offsets), _ptr(w.data),
         _ptr(out), 1 if out_dtype == torch.float32 else 0, w.halves - 1,
         0 if offsets is not None else num_rows, w.cols, x.shape[1], w.experts, w.group_size,
         rows_per_pass, active, 1 if offsets_settled else 0, _ptr(row_scale),
@@ -1690,8 +1688,13 @@ def _int4_tc(what, x, rows, offsets, w, num_rows, out_dtype, row_scale=None, act
     elif rows is not None:
         x = gather_rows(x, rows)
     out = torch.empty((num_rows, w.cols), dtype=out_dtype, device=x.device)
-    _check(_lib().ix_int4_tc(
-        _ptr(x), terms, _ptr(offsets), _ptr(w.codes), _ptr(w.params), _ptr(out),
+    lib = _lib()
+    lib.ix_int4_tc_scratch.restype = ctypes.c_longlong
+    need = lib.ix_int4_tc_scratch(num_rows, w.cols, x.shape[-1], w.experts,
+                                  0 if offsets is None else 1, w.halves - 1, terms)
+    part = torch.empty(need, dtype=torch.float32, device=x.device) if need else None
+    _check(lib.ix_int4_tc(
+        _ptr(x), terms, _ptr(offsets), _ptr(w.data), _ptr(out), _ptr(part),
         1 if out_dtype == torch.float32 else 0, w.halves - 1, num_rows, w.cols, x.shape[-1],
         w.experts, w.group_size, _ptr(row_scale), _ACTIVATIONS[activation],
         _ptr(_tc_status(x.device)), _stream()), what)
