@@ -11,7 +11,7 @@
 // (cta_group::2): 256 weight rows (DUAL: 128 gate rows and the up rows of the same columns) for a tile
 // of up to BT rows of one expert, over all of K or one of `splits` runs of it.  A block holds 128 of the
 // weight rows and half of the tile's rows, so each of the two halves is brought once.  Pairs are
-// persistent and take items round robin.  Roles of a block's sixteen warps, a chunk of 128 k at a time:
+// persistent and take items round robin.  Roles of a block's twenty warps, a chunk of 128 k at a time:
 //   0      brings the rows into a ring of stages (TMA, 128-byte swizzle);
 //   1      the first block's issues the MMAs for both, a group of k into one of two accumulators in
 //          tensor memory; the second block's tells the first that its own operands are there;
@@ -20,7 +20,7 @@
 //          sum to fp32 registers;
 //          Rows of a DUAL item lie as 16 gate rows, the 16 up rows of the same columns, and so on, so
 //          that a column's two sums are sixteen lanes of one warp apart;
-//   12-15  unpack: a lane's 16 bytes of codes are eight neighbouring k of two rows, twice; less their
+//   12-19  unpack a strip each: a lane's 16 bytes of codes are eight neighbouring k of two rows, twice; less their
 //          zero points they are whole numbers, written as a swizzled operand tile.
 // So the operands of the tensor cores are exact (a code less its zero point has five bits), the sums of
 // a group are the tensor cores' fp32, and a group's scale multiplies in fp32: no weight is rounded to
@@ -34,9 +34,11 @@
 #include "tcgen05_common.cuh"
 #include "tma_common.cuh"
 
-#define I4T_THREADS 512
+#define I4T_THREADS 640
 #define I4T_TILE (128 * 64 * 2)           // 64 k of a block's weight rows, unpacked
 #define I4T_MAX_EXPERTS 1024              // the prefix of tiles lives in shared memory
+#define I4T_NAP 20000                     // ns
+#define I4T_WAIT_CLOCKS 4000000000LL      // about two seconds
 #define I4T_DONE 4                        // barriers of finished chunks
 
 enum {
@@ -67,8 +69,8 @@ template <int TERMS, bool DUAL, int BT, int GROUP> struct I4TCfg {
   static constexpr int X_STAGE = TERMS * 2 * X_TILE;
   static constexpr int BOX = BT / 4;                           // rows of a TMA box
   static constexpr int C_BYTES = i4_block_words(GROUP) * 4;    // a strip's codes and parameters
-  static constexpr int X_RING = TERMS == 3 ? 2 : 4;
-  static constexpr int A_RING = BT == 128 && TERMS == 1 ? 3 : 2;
+  static constexpr int X_RING = TERMS == 3 ? 2 : BT == 256 ? 3 : 4;
+  static constexpr int A_RING = TERMS == 3 ? 2 : 3;
   static constexpr int C_RING = BT == 128 ? 4 : 2;
   // Scales are written once the MMAs of A_RING chunks before have run, and those had waited for the
   // sums of two chunks before them to be taken: a slot is read by then.
@@ -90,22 +92,32 @@ __device__ __forceinline__ void i4t_copy(void* to, const void* from, unsigned by
       "l"(from), "r"(bytes), "r"(smem_u32(bar))
       : "memory");
 }
-// mbar_wait for what the other block of the pair has written.  (A fence.acq_rel.cluster behind a wait
-// of the block's own scope took 1,000 cycles a chunk.)
-__device__ __forceinline__ bool i4t_wait_cluster(unsigned long long* bar, unsigned parity,
-                                                 volatile int* abort_flag) {
-  for (int i = 0; i < IX_WAIT_POLLS; ++i) {
-    unsigned ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity)
-        : "memory");
-    if (ok) return true;
+// Arrives at a barrier of the other block.  Of the block's own scope, as the waits behind it are: what
+// it announces is read by MMAs, by the asynchronous proxy that the operands' writers have fenced theirs
+// into, and not by loads of a thread.  (Released at cluster scope an arrival takes some 1,400 cycles,
+// more than a chunk's MMAs.)
+__device__ __forceinline__ void i4t_arrive_at(unsigned bar) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// Bounded wait; its polls sleep in the barrier unit, up to I4T_NAP ns each.
+__device__ __forceinline__ bool i4t_try(unsigned long long* bar, unsigned parity) {
+  unsigned ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity), "r"(I4T_NAP)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ bool i4t_wait(unsigned long long* bar, unsigned parity,
+                                         volatile int* abort_flag) {
+  if (i4t_try(bar, parity)) return true;
+  const long long begin = clock64();
+  while (clock64() - begin < I4T_WAIT_CLOCKS) {
+    if (i4t_try(bar, parity)) return true;
     if (*abort_flag) return false;
-    if (i > 1024) __nanosleep(64);
   }
   return false;
 }
@@ -209,13 +221,13 @@ int4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
   }
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::X_RING; ++s) mbar_init(&full_x[s], 1);
-    for (int s = 0; s < C::A_RING; ++s) mbar_init(&full_a[s], 4);
+    for (int s = 0; s < C::A_RING; ++s) mbar_init(&full_a[s], 8);
     for (int s = 0; s < C::C_RING; ++s) {
       mbar_init(&full_c[s], 1);
-      mbar_init(&empty_c[s], 4);
+      mbar_init(&empty_c[s], 8);
     }
     for (int s = 0; s < I4T_DONE; ++s) mbar_init(&done[s], 1);
-    for (int s = 0; s < C::S_RING; ++s) mbar_init(&full_s[s], 4);
+    for (int s = 0; s < C::S_RING; ++s) mbar_init(&full_s[s], 8);
     for (int b = 0; b < 2; ++b) {
       mbar_init(&acc_full[b], 1);
       mbar_init(&acc_empty[b], 8);
@@ -269,13 +281,13 @@ int4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
     return it;
   };
   auto wait = [&](unsigned long long* bar, int parity) {
-    return (bool)__all_sync(0xffffffffu, mbar_wait(bar, parity, abortp));
+    return (bool)__all_sync(0xffffffffu, i4t_wait(bar, parity, abortp));
   };
 
-  // Registers go from the roles that need few to the warps that hold up to 128 sums a lane (512
-  // threads at 128: 128 x 40 + 256 x 200 + 128 x 72).
+  // Registers go from the roles that need few to the warps that hold up to 128 sums a lane (640
+  // threads at 96: 128 x 32 + 256 x 168 + 256 x 56).
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");
     if (warp == 0) {
       int n = 0;                             // chunks so far, over all items
       bool ok = true;
@@ -331,12 +343,11 @@ int4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
             ok = wait(&acc_empty[buf], (group >> 1 & 1) ^ 1);
             if (!ok) break;
             if (rank != 0) {
-              if (lane == 0) tc_arrive_at(peer_at + (group & 3) * 8);
+              if (lane == 0) i4t_arrive_at(peer_at + (group & 3) * 8);
               __syncwarp();
               continue;
             }
-            ok = (bool)__all_sync(0xffffffffu,
-                                  i4t_wait_cluster(&peer[group & 3], group >> 2 & 1, abortp));
+            ok = wait(&peer[group & 3], group >> 2 & 1);
             if (!ok) break;
             tc_fence_after();
             const unsigned sums = tmem_base + buf * BT;
@@ -396,10 +407,12 @@ int4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
       }
     }
   } else if (warp >= 12) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-    const int unpacker = warp - 12;          // strips 2 u and 2 u + 1
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    const int unpacker = warp - 12;          // its strip (DUAL: gate strips are 0, 2, 4, 6)
     const int g = lane >> 2, t = lane & 3;
     const bool odd = g & 1;
+    // (DUAL: four gate strips were copied, then four up strips)
+    const int from = DUAL ? (unpacker & 1) * 4 + (unpacker >> 1) : unpacker;
     int n = 0;
     bool ok = true;
     for (int w = first; w < n_items && ok; w += step) {
@@ -409,20 +422,15 @@ int4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
         const int sc = n % C::C_RING, sa = n % C::A_RING;
         ok = wait(&full_c[sc], n / C::C_RING & 1);
         if (!ok) break;
-        uint4 code[2][2];
-        unsigned pa[2][NG], pb[2][NG];
+        const unsigned* own = reinterpret_cast<const unsigned*>(cs + (sc * 8 + from) * C::C_BYTES);
+        uint4 code[2];
+        unsigned pa[NG], pb[NG];
+        code[0] = *reinterpret_cast<const uint4*>(own + lane * 4);
+        code[1] = *reinterpret_cast<const uint4*>(own + I4_TILE_WORDS + lane * 4);
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          // (DUAL: four gate strips were copied, then four up strips)
-          const unsigned* own = reinterpret_cast<const unsigned*>(
-              cs + (sc * 8 + (DUAL ? u * 4 + unpacker : unpacker * 2 + u)) * C::C_BYTES);
-          code[u][0] = *reinterpret_cast<const uint4*>(own + lane * 4);
-          code[u][1] = *reinterpret_cast<const uint4*>(own + I4_TILE_WORDS + lane * 4);
-#pragma unroll
-          for (int i = 0; i < NG; ++i) {
-            pa[u][i] = own[I4_CODE_WORDS + g * NG + i];
-            pb[u][i] = own[I4_CODE_WORDS + (g + 8) * NG + i];
-          }
+        for (int i = 0; i < NG; ++i) {
+          pa[i] = own[I4_CODE_WORDS + g * NG + i];
+          pb[i] = own[I4_CODE_WORDS + (g + 8) * NG + i];
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&empty_c[sc]);
@@ -433,52 +441,48 @@ int4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
         }
         // the scales, by row and group, to the warps that add up
         if (t == 0) {
+          unsigned short* to = scales + ((n % C::S_RING) * 128 + unpacker * 16 + g) * NG;
+          i4t_scales<NG>(to, pa);
+          i4t_scales<NG>(to + 8 * NG, pb);
+        }
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            unsigned short* to = scales + ((n % C::S_RING) * 128 + (unpacker * 2 + u) * 16 + g) * NG;
-            i4t_scales<NG>(to, pa[u]);
-            i4t_scales<NG>(to + 8 * NG, pb[u]);
+        for (int h = 0; h < 2; ++h) {
+          unsigned char* at = as + (sa * 2 + h) * I4T_TILE + unpacker * 2048 + g * 128;
+#pragma unroll
+          for (int run = 0; run < 2; ++run) {
+            // lanes of odd rows take the two runs of eight k the other way round, so that the
+            // eight lanes of a store phase meet all banks
+            const bool second = (run == 1) != odd;
+            const unsigned w0 = second ? code[h].z : code[h].x;
+            const unsigned w1 = second ? code[h].w : code[h].y;
+            unsigned sa2, sb2;
+            if (GROUP == 32) {
+              sa2 = i4_sub(second ? pa[(2 * h + 1) % NG] : pa[2 * h % NG]);
+              sb2 = i4_sub(second ? pb[(2 * h + 1) % NG] : pb[2 * h % NG]);
+            } else {
+              sa2 = i4_sub(pa[GROUP == 64 ? h % NG : 0]);
+              sb2 = i4_sub(pb[GROUP == 64 ? h % NG : 0]);
+            }
+            const int where = (((second ? 4 : 0) + t) ^ g) * 16;
+            *reinterpret_cast<uint4*>(at + where) =
+                make_uint4(i4_pair(w0, 0, sa2), i4_pair(w0, 2, sa2), i4_pair(w1, 0, sa2),
+                           i4_pair(w1, 2, sa2));
+            *reinterpret_cast<uint4*>(at + 1024 + where) =
+                make_uint4(i4_pair(w0, 1, sb2), i4_pair(w0, 3, sb2), i4_pair(w1, 1, sb2),
+                           i4_pair(w1, 3, sb2));
           }
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&full_s[n % C::S_RING]);
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            unsigned char* at = as + (sa * 2 + h) * I4T_TILE + (unpacker * 2 + u) * 2048 + g * 128;
-#pragma unroll
-            for (int run = 0; run < 2; ++run) {
-              // lanes of odd rows take the two runs of eight k the other way round, so that the
-              // eight lanes of a store phase meet all banks
-              const bool second = (run == 1) != odd;
-              const unsigned w0 = second ? code[u][h].z : code[u][h].x;
-              const unsigned w1 = second ? code[u][h].w : code[u][h].y;
-              unsigned sa2, sb2;
-              if (GROUP == 32) {
-                sa2 = i4_sub(second ? pa[u][(2 * h + 1) % NG] : pa[u][2 * h % NG]);
-                sb2 = i4_sub(second ? pb[u][(2 * h + 1) % NG] : pb[u][2 * h % NG]);
-              } else {
-                sa2 = i4_sub(pa[u][GROUP == 64 ? h % NG : 0]);
-                sb2 = i4_sub(pb[u][GROUP == 64 ? h % NG : 0]);
-              }
-              const int where = (((second ? 4 : 0) + t) ^ g) * 16;
-              *reinterpret_cast<uint4*>(at + where) =
-                  make_uint4(i4_pair(w0, 0, sa2), i4_pair(w0, 2, sa2), i4_pair(w1, 0, sa2),
-                             i4_pair(w1, 2, sa2));
-              *reinterpret_cast<uint4*>(at + 1024 + where) =
-                  make_uint4(i4_pair(w0, 1, sb2), i4_pair(w0, 3, sb2), i4_pair(w1, 1, sb2),
-                             i4_pair(w1, 3, sb2));
-            }
-          }
         fence_proxy_async();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&full_a[sa]);
+        if (lane == 0) {
+          mbar_arrive(&full_a[sa]);
+          mbar_arrive(&full_s[n % C::S_RING]);
+        }
       }
     }
     if (!ok && lane == 0 && !*abortp) { atomicExch(p.status, I4T_ERR_UNPACK); *abortp = 1; }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
     const int quarter = warp & 3, half = (warp - 4) >> 2;  // lanes of tensor memory; every second 32 rows
     const unsigned lanes = tmem_base + ((unsigned)(quarter * 32) << 16);
     int n = 0, group = 0;
