@@ -30,6 +30,8 @@
 // Every wait on an mbarrier is bounded: the waiter records a code in `status` (51 and 54 copies, 52
 // MMAs, 53 unpacking, 55 sums), raises a flag that ends its block's other roles, and the pair meets at
 // its end, where tensor memory is freed.
+#include <type_traits>
+
 #include "int4_format.cuh"
 #include "tcgen05_common.cuh"
 #include "tma_common.cuh"
@@ -49,7 +51,7 @@ struct I4TArgs {
   const int* offsets;       // null: one matrix with `rows` rows
   const unsigned* data;
   void* out;
-  float* part;              // splits > 1: [splits][rows][columns of both halves] sums
+  float* part;              // splits > 1, or an activation: [splits][rows][columns of both halves] sums
   int wide;                 // fp32 results, otherwise bfloat16
   const float* row_scale;
   int plain;
@@ -144,30 +146,16 @@ template <int NG> __device__ __forceinline__ void i4t_scales(unsigned short* to,
         make_uint2(__byte_perm(v[0], v[NG > 1 ? 1 : 0], 0x5410),
                    __byte_perm(v[NG > 2 ? 2 : 0], v[NG - 1], 0x5410));
 }
-// Out of line: an epilogue that holds them unrolled runs from a cold instruction cache.
-__device__ __noinline__ float i4t_act(float v, int act, int wide) {
-  return wide ? ix_act<float>(v, act) : ix_act<bf16>(v, act);
-}
+// Out of line: an epilogue that holds it unrolled runs from a cold instruction cache.
 __device__ __noinline__ float i4t_silu_wide(float a, float u) { return a / (1.0f + expf(-a)) * u; }
 
-// Up to ROWS rows of one column (the first at entry `at` of the result).
-template <int ROWS>
-__device__ __forceinline__ void i4t_store(const I4TArgs& p, float* v, int n, size_t at) {
-  if (p.plain) {
+// sum += scale * (32 columns of this thread's lane)
+__device__ __forceinline__ void i4t_add(unsigned long long* sum, unsigned long long scale,
+                                        unsigned taddr) {
+  float v[32];
+  tc_ld32(taddr, v);
 #pragma unroll
-    for (int j = 0; j < ROWS; ++j) v[j] = i4t_act(v[j], p.plain, p.wide);
-  }
-  if (p.wide) {
-    float* o = (float*)p.out + at;
-#pragma unroll
-    for (int j = 0; j < ROWS; ++j)
-      if (j < n) o[(size_t)j * p.N] = v[j];
-  } else {
-    bf16* o = (bf16*)p.out + at;
-#pragma unroll
-    for (int j = 0; j < ROWS; ++j)
-      if (j < n) o[(size_t)j * p.N] = __float2bfloat16_rn(v[j]);
-  }
+  for (int j = 0; j < 16; ++j) i4t_fma2(sum[j], scale, i4t_pack(v[2 * j], v[2 * j + 1]));
 }
 
 template <int BT>
@@ -185,12 +173,15 @@ int4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
   unsigned char* as = xs + C::X_RING * C::X_STAGE;
   unsigned char* cs = as + C::A_RING * 2 * I4T_TILE;
   unsigned short* scales = reinterpret_cast<unsigned short*>(cs + C::C_RING * 8 * C::C_BYTES);
-  __shared__ __align__(8) unsigned long long full_x[C::X_RING], full_a[C::A_RING];
+  // A group may be multiplied: on a chunk's first group the block's operands are there (eight unpacking
+  // warps and the rows' bytes), an accumulator's sums are taken (eight warps), and, in the first block,
+  // the second one is as far.  One barrier for all of it, as a wait costs the issuing warp hundreds of
+  // cycles even where nothing is waited for.
+  __shared__ __align__(8) unsigned long long go[I4T_DONE][NG];
   __shared__ __align__(8) unsigned long long full_c[C::C_RING], empty_c[C::C_RING];
   __shared__ __align__(8) unsigned long long done[I4T_DONE];     // a chunk's MMAs have run
   __shared__ __align__(8) unsigned long long full_s[C::S_RING];  // a chunk's scales are there
-  __shared__ __align__(8) unsigned long long acc_full[2], acc_empty[2];
-  __shared__ __align__(8) unsigned long long peer[4];            // the second block is ready for a group
+  __shared__ __align__(8) unsigned long long acc_full[2];
   __shared__ unsigned tmem_holder;
   __shared__ int abort_flag;
   __shared__ int tile_start[I4T_MAX_EXPERTS + 1];
@@ -220,19 +211,15 @@ int4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
     }
   }
   if (threadIdx.x == 0) {
-    for (int s = 0; s < C::X_RING; ++s) mbar_init(&full_x[s], 1);
-    for (int s = 0; s < C::A_RING; ++s) mbar_init(&full_a[s], 8);
+    for (int s = 0; s < I4T_DONE; ++s)
+      for (int q = 0; q < NG; ++q) mbar_init(&go[s][q], (q == 0 ? 17 : 8) + (rank == 0 ? 1 : 0));
     for (int s = 0; s < C::C_RING; ++s) {
       mbar_init(&full_c[s], 1);
       mbar_init(&empty_c[s], 8);
     }
     for (int s = 0; s < I4T_DONE; ++s) mbar_init(&done[s], 1);
     for (int s = 0; s < C::S_RING; ++s) mbar_init(&full_s[s], 8);
-    for (int b = 0; b < 2; ++b) {
-      mbar_init(&acc_full[b], 1);
-      mbar_init(&acc_empty[b], 8);
-    }
-    for (int b = 0; b < 4; ++b) mbar_init(&peer[b], 1);
+    for (int b = 0; b < 2; ++b) mbar_init(&acc_full[b], 1);
     abort_flag = 0;
     mbar_init_fence();
     fence_proxy_async();
@@ -306,24 +293,28 @@ int4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
             if (!ok) break;
           }
           if (lane == 0)
-            mbar_expect_tx(&full_x[s], (unsigned)(TERMS * 2 * boxes * C::BOX * 64 * 2));
+            mbar_expect_tx(&go[n % I4T_DONE][0], (unsigned)(TERMS * 2 * boxes * C::BOX * 64 * 2));
           __syncwarp();
           if (term < TERMS)
             tma_load_2d(xs + s * C::X_STAGE + (term * 2 + sub) * C::X_TILE +
                             box * (C::BOX * 64 * 2),
                         &map_x, c * 128 + sub * 64,
-                        term * p.plane_rows + it.m0 + rank * half + box * C::BOX, &full_x[s]);
+                        term * p.plane_rows + it.m0 + rank * half + box * C::BOX,
+                        &go[n % I4T_DONE][0]);
           __syncwarp();
         }
       }
       if (lane == 0) {
         if (!ok && !*abortp) { atomicExch(p.status, I4T_ERR_COPY); *abortp = 1; }
         // copies in flight land before the block's shared memory goes away, whatever the others do
-        for (int f = max(0, n - C::X_RING); f < n; ++f)
-          mbar_drain(&full_x[f % C::X_RING], f / C::X_RING & 1);
+        if (!ok)
+          for (int f = max(0, n - C::X_RING); f < n; ++f)
+            mbar_drain(&go[f % I4T_DONE][0], f / I4T_DONE & 1);
+        else if (n > 0)
+          mbar_drain(&done[(n - 1) % I4T_DONE], (n - 1) / I4T_DONE & 1);
       }
     } else if (warp == 1) {
-      const unsigned peer_at = tc_of_rank(&peer[0], 0);
+      const unsigned first_block = tc_of_rank(&go[0][0], 0);
       int n = 0, group = 0;
       bool ok = true;
       for (int w = first; w < n_items && ok; w += step) {
@@ -333,23 +324,19 @@ int4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
         const unsigned idesc = (1u << 4) | (1u << 7) | (1u << 10) |
                                ((unsigned)(((it.n + 31) & ~31) >> 3) << 17) | (16u << 24);
         for (int c = it.c0; c < it.c1 && ok; ++c, ++n) {
-          const int sx = n % C::X_RING, sa = n % C::A_RING;
-          ok = wait(&full_a[sa], n / C::A_RING & 1) && wait(&full_x[sx], n / C::X_RING & 1);
-          if (!ok) break;
-          const unsigned long long ad = umma_desc(as + sa * 2 * I4T_TILE);
-          const unsigned long long xd = umma_desc(xs + sx * C::X_STAGE);
-          for (int q = 0; q < NG && ok; ++q, ++group) {
-            const int buf = group & 1;
-            ok = wait(&acc_empty[buf], (group >> 1 & 1) ^ 1);
+          const int slot = n % I4T_DONE;
+          const unsigned long long ad = umma_desc(as + (n % C::A_RING) * 2 * I4T_TILE);
+          const unsigned long long xd = umma_desc(xs + (n % C::X_RING) * C::X_STAGE);
+          for (int q = 0; q < NG; ++q, ++group) {
+            ok = wait(&go[slot][q], n / I4T_DONE & 1);
             if (!ok) break;
             if (rank != 0) {
-              if (lane == 0) i4t_arrive_at(peer_at + (group & 3) * 8);
+              if (lane == 0) i4t_arrive_at(first_block + (slot * NG + q) * 8);
               __syncwarp();
               continue;
             }
-            ok = wait(&peer[group & 3], group >> 2 & 1);
-            if (!ok) break;
             tc_fence_after();
+            const int buf = group & 1;
             const unsigned sums = tmem_base + buf * BT;
             if (lane == 0) {
 #pragma unroll
@@ -364,7 +351,7 @@ int4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
                               i == 0 && t == TERMS - 1 ? 0u : 1u);
               }
               if (NG > 1) tc_commit_pair(&acc_full[buf]);
-              if (q == NG - 1) tc_commit_pair(&done[n % I4T_DONE]);
+              if (q == NG - 1) tc_commit_pair(&done[slot]);
             }
             __syncwarp();
           }
@@ -475,7 +462,7 @@ int4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
         fence_proxy_async();
         __syncwarp();
         if (lane == 0) {
-          mbar_arrive(&full_a[sa]);
+          mbar_arrive(&go[n % I4T_DONE][0]);
           mbar_arrive(&full_s[n % C::S_RING]);
         }
       }
@@ -487,6 +474,12 @@ int4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
     const unsigned lanes = tmem_base + ((unsigned)(quarter * 32) << 16);
     int n = 0, group = 0;
     bool ok = true;
+    // group g's accumulator is free
+    auto free_for = [&](int g) {
+      if (lane == 0) mbar_arrive(&go[g / NG % I4T_DONE][g % NG]);
+    };
+    free_for(0);
+    free_for(1);
     unsigned long long sum[BT / 64][16];     // pairs of rows
     for (int w = first; w < n_items && ok; w += step) {
       const I4TItem it = item_of(w);
@@ -511,26 +504,26 @@ int4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
                        : wait(&acc_full[buf], group >> 1 & 1);
           if (!ok) break;
           tc_fence_after();
+          // (a tile that fills its columns takes them without a branch between)
+          if (it.n > BT - 64) {
 #pragma unroll
-          for (int i = 0; i < BT / 64; ++i) {
-            const int col = 64 * i + 32 * half;
-            if (col < it.n) {
-              float v[32];
-              tc_ld32(lanes + buf * BT + col, v);
+            for (int i = 0; i < BT / 64; ++i)
+              i4t_add(sum[i], scale[q], lanes + buf * BT + 64 * i + 32 * half);
+          } else {
 #pragma unroll
-              for (int j = 0; j < 16; ++j)
-                i4t_fma2(sum[i][j], scale[q], i4t_pack(v[2 * j], v[2 * j + 1]));
-            }
+            for (int i = 0; i < BT / 64 - 1; ++i)
+              if (64 * i + 32 * half < it.n)
+                i4t_add(sum[i], scale[q], lanes + buf * BT + 64 * i + 32 * half);
           }
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&acc_empty[buf]);
+          free_for(group + 2);
         }
       }
       if (!ok) break;
       // -- a lane holds one weight row for 32 rows at a time: 64- or 128-byte stores of a warp
       const int f_own = it.f0 + rank * (F / 2);
-      if (p.splits > 1) {
+      if (p.part) {
         // sums of a run of K: the halves' columns beside each other
         const int f = DUAL ? f_own + quarter * 16 + (lane & 15) : f_own + quarter * 32 + lane;
         const size_t width = DUAL ? 2 * (size_t)p.N : (size_t)p.N;
@@ -553,44 +546,76 @@ int4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
         // up sums the second: each gets the other sum of its row
         const bool up = lane >= 16;
         const int f = f_own + quarter * 16 + (lane & 15);
+        auto finish = [&](auto wide, auto scaled) {
 #pragma unroll
-        for (int i = 0; i < BT / 64; ++i) {
-          const int col = 64 * i + 32 * half + (up ? 1 : 0);
-          if (64 * i + 32 * half >= it.n) continue;
-          const int n_here = f < p.N ? it.n - col : 0;
-          const size_t at = (size_t)(it.m0 + col) * p.N + f;
+          for (int i = 0; i < BT / 64; ++i) {
+            const int col = 64 * i + 32 * half + (up ? 1 : 0);
+            if (64 * i + 32 * half >= it.n) continue;
+            const int n_here = f < p.N ? it.n - col : 0;
+            const size_t at = (size_t)(it.m0 + col) * p.N + f;
+            const size_t two = 2 * (size_t)p.N;
+            float* o = (float*)p.out + at;
+            bf16* ob = (bf16*)p.out + at;
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            float first_row, second_row;
-            i4t_unpack(sum[i][j], first_row, second_row);
-            const float got = __shfl_xor_sync(0xffffffffu, up ? first_row : second_row, 16);
-            float a = up ? got : first_row, u = up ? second_row : got;
-            if (p.row_scale) {
-              const float s = 2 * j < n_here ? p.row_scale[it.m0 + col + 2 * j] : 0.f;
-              a *= s;
-              u *= s;
-            }
-            if (p.wide) {
-              const float y = i4t_silu_wide(a, u);
-              if (2 * j < n_here) ((float*)p.out)[at + (size_t)(2 * j) * p.N] = y;
-            } else {
-              const float y = __fdividef(a, 1.0f + __expf(-a)) * u;
-              if (2 * j < n_here)
-                ((bf16*)p.out)[at + (size_t)(2 * j) * p.N] = __float2bfloat16_rn(y);
+            for (int j = 0; j < 16; ++j) {
+              float first_row, second_row;
+              i4t_unpack(sum[i][j], first_row, second_row);
+              const float got = __shfl_xor_sync(0xffffffffu, up ? first_row : second_row, 16);
+              float a = up ? got : first_row, u = up ? second_row : got;
+              if (scaled.value) {
+                const float s = 2 * j < n_here ? p.row_scale[it.m0 + col + 2 * j] : 0.f;
+                a *= s;
+                u *= s;
+              }
+              if (wide.value) {
+                const float y = i4t_silu_wide(a, u);
+                if (2 * j < n_here) *o = y;
+                o += two;
+              } else {
+                const float y = __fdividef(a, 1.0f + __expf(-a)) * u;
+                if (2 * j < n_here) *ob = __float2bfloat16_rn(y);
+                ob += two;
+              }
             }
           }
+        };
+        if (p.wide) {
+          if (p.row_scale) finish(std::true_type(), std::true_type());
+          else finish(std::true_type(), std::false_type());
+        } else {
+          if (p.row_scale) finish(std::false_type(), std::true_type());
+          else finish(std::false_type(), std::false_type());
         }
       } else {
         const int f = f_own + quarter * 32 + lane;
+        auto finish = [&](auto wide) {
 #pragma unroll
-        for (int i = 0; i < BT / 32; ++i) {            // sixteen rows at a time
-          const int col = 64 * (i >> 1) + 32 * half + 16 * (i & 1);
-          if (col >= it.n) continue;
-          float v[16];
+          for (int i = 0; i < BT / 64; ++i) {
+            const int col = 64 * i + 32 * half;
+            if (col >= it.n) continue;
+            const int n_here = f < p.N ? it.n - col : 0;
+            const size_t at = (size_t)(it.m0 + col) * p.N + f;
+            float* o = (float*)p.out + at;
+            bf16* ob = (bf16*)p.out + at;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) i4t_unpack(sum[i >> 1][8 * (i & 1) + j], v[2 * j], v[2 * j + 1]);
-          i4t_store<16>(p, v, f < p.N ? it.n - col : 0, (size_t)(it.m0 + col) * p.N + f);
-        }
+            for (int j = 0; j < 16; ++j) {
+              float y[2];
+              i4t_unpack(sum[i][j], y[0], y[1]);
+#pragma unroll
+              for (int k = 0; k < 2; ++k) {
+                if (wide.value) {
+                  if (2 * j + k < n_here) *o = y[k];
+                  o += p.N;
+                } else {
+                  if (2 * j + k < n_here) *ob = __float2bfloat16_rn(y[k]);
+                  ob += p.N;
+                }
+              }
+            }
+          }
+        };
+        if (p.wide) finish(std::true_type());
+        else finish(std::false_type());
       }
     }
     if (!ok && lane == 0 && !*abortp) { atomicExch(p.status, I4T_ERR_SUM); *abortp = 1; }
@@ -607,26 +632,27 @@ template <bool DUAL>
 __global__ void __launch_bounds__(256)
 int4_join_kernel(const I4TArgs p) {
   const int f = blockIdx.x * 256 + threadIdx.x;
-  const size_t r = blockIdx.y;
   if (f >= p.N) return;
   const size_t width = DUAL ? 2 * (size_t)p.N : (size_t)p.N, plane = (size_t)p.rows * width;
-  const float* from = p.part + r * width + f;
-  float a = 0.f, u = 0.f;
-  for (int z = 0; z < p.splits; ++z, from += plane) {
-    a += from[0];
-    if (DUAL) u += from[p.N];
-  }
-  if (DUAL) {
-    if (p.row_scale) {
-      a *= p.row_scale[r];
-      u *= p.row_scale[r];
+  for (size_t r = blockIdx.y; r < (size_t)p.rows; r += gridDim.y) {
+    const float* from = p.part + r * width + f;
+    float a = 0.f, u = 0.f;
+    for (int z = 0; z < p.splits; ++z, from += plane) {
+      a += from[0];
+      if (DUAL) u += from[p.N];
     }
-    a = p.wide ? a / (1.0f + expf(-a)) * u : __fdividef(a, 1.0f + __expf(-a)) * u;
-  } else if (p.plain) {
-    a = p.wide ? ix_act<float>(a, p.plain) : ix_act<bf16>(a, p.plain);
+    if (DUAL) {
+      if (p.row_scale) {
+        a *= p.row_scale[r];
+        u *= p.row_scale[r];
+      }
+      a = p.wide ? a / (1.0f + expf(-a)) * u : __fdividef(a, 1.0f + __expf(-a)) * u;
+    } else if (p.plain) {
+      a = p.wide ? ix_act<float>(a, p.plain) : ix_act<bf16>(a, p.plain);
+    }
+    if (p.wide) ((float*)p.out)[r * p.N + f] = a;
+    else ((bf16*)p.out)[r * p.N + f] = __float2bfloat16_rn(a);
   }
-  if (p.wide) ((float*)p.out)[r * p.N + f] = a;
-  else ((bf16*)p.out)[r * p.N + f] = __float2bfloat16_rn(a);
 }
 
 template <int TERMS, bool DUAL, int BT, int GROUP>
@@ -644,8 +670,9 @@ static int i4t_launch(const void* x, int Kp, const I4TArgs& p, int sms, cudaStre
   if (e != cudaSuccess) return (int)e;
   const int pairs = sms / 2;
   kern<<<2 * (int)(items < pairs ? items : pairs), I4T_THREADS, C::SMEM, stream>>>(map, p);
-  if (p.splits > 1)
-    int4_join_kernel<DUAL><<<dim3((p.N + 255) / 256, p.rows), 256, 0, stream>>>(p);
+  if (p.part)
+    int4_join_kernel<DUAL><<<dim3((p.N + 255) / 256, p.rows < 16384 ? p.rows : 16384), 256, 0,
+                             stream>>>(p);
   return ix_launch_status();
 }
 
@@ -703,10 +730,11 @@ static I4TPlan i4t_plan(int rows, int N, int Kp, int E, bool grouped, bool dual,
 }
 
 // fp32 entries of scratch that a call of these sizes wants (0: none)
-IX_API long long ix_int4_tc_scratch(int rows, int N, int Kp, int E, int grouped, int dual, int terms) {
+IX_API long long ix_int4_tc_scratch(int rows, int N, int Kp, int E, int grouped, int dual, int terms,
+                                    int plain) {
   if (rows <= 0 || N <= 0 || Kp <= 0 || E <= 0) return 0;
   const I4TPlan plan = i4t_plan(rows, N, Kp, E, grouped != 0, dual != 0, terms);
-  return plan.splits > 1 ? (long long)plan.splits * rows * N * (dual ? 2 : 1) : 0;
+  return plan.splits > 1 || plain ? (long long)plan.splits * rows * N * (dual ? 2 : 1) : 0;
 }
 
 // x: [rows, Kp] bf16, or [3, rows, Kp] terms of fp32 rows; Kp a multiple of 8 that ends in the last
@@ -723,7 +751,11 @@ IX_API int ix_int4_tc(const void* x, int terms, const int* offsets, const void* 
   if (((uintptr_t)x | (uintptr_t)data) & 15) return IX_ERR_ALIGN;
   if (3LL * rows > 0x7fffffffLL || N > 0x3fffff00) return IX_ERR_SIZE;
   const I4TPlan plan = i4t_plan(rows, N, Kp, E, offsets != nullptr, dual != 0, terms);
-  if (plan.splits > 1 && (part == nullptr || rows > 65535)) return IX_ERR_SIZE;
+  if (plan.splits > 1 || plain) {
+    if (part == nullptr) return IX_ERR_SIZE;
+  } else {
+    part = nullptr;
+  }
   const int chunks = (int)i4_chunks(Kp);
   const I4TArgs p = {offsets, (const unsigned*)data, out, part, wide, row_scale, plain, rows, N,
                      (int)i4_strips(N), chunks, E, plan.tile_rows, plan.splits,

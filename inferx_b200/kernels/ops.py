@@ -1691,7 +1691,8 @@ def _int4_tc(what, x, rows, offsets, w, num_rows, out_dtype, row_scale=None, act
     lib = _lib()
     lib.ix_int4_tc_scratch.restype = ctypes.c_longlong
     need = lib.ix_int4_tc_scratch(num_rows, w.cols, x.shape[-1], w.experts,
-                                  0 if offsets is None else 1, w.halves - 1, terms)
+                                  0 if offsets is None else 1, w.halves - 1, terms,
+                                  _ACTIVATIONS[activation])
     part = torch.empty(need, dtype=torch.float32, device=x.device) if need else None
     _check(lib.ix_int4_tc(
         _ptr(x), terms, _ptr(offsets), _ptr(w.data), _ptr(out), _ptr(part),
