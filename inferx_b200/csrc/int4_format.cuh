@@ -8,12 +8,11 @@
 // strips that a tile of weight rows takes of a chunk are one piece of memory (one bulk copy), and a
 // strip's share of it is 1 KB and its parameters.
 //
-// Codes.  [tile of 64 k][lane 0..31][word 0..3].  Lane 4 g + t holds rows g and g + 8 for the k of two
-// runs of eight, 8 t .. 8 t + 7 and 32 + 8 t .. 32 + 8 t + 7; word 2 h + j has the entries 4 j .. 4 j + 3
-// of run h.  Nibbles i and i + 4 of a word are a pair of neighbouring k: i = 0, 1: the first pair of
-// rows g and g + 8; i = 2, 3: the second.  So 16 bytes of a lane are the A side of four mma.m16n8k16
-// (k in an order that the activations' 16-byte loads follow too), and the four lanes of a row hold
-// 16-byte pieces that lie beside each other in a K-major operand tile.
+// Codes.  [tile of 64 k][lane 0..31][word 0..3].  Word j of lane 4 g + t has the entries k = 16 j +
+// 4 t .. + 3 of rows g and g + 8.  Nibbles i and i + 4 of a word are a pair of neighbouring k: i = 0, 1:
+// the first pair of rows g and g + 8; i = 2, 3: the second.  So a word is the A side of one
+// mma.m16n8k16 (k in an order that the activations' 8-byte loads follow too), and, as four registers of
+// pairs, sixteen rows by sixteen k of an operand in tensor memory (the 16x256b shape).
 //
 // Parameters.  [row 0..15][group of the chunk]: one word, the scale in the low half, 128 + zero as
 // bfloat16 in the high half.  (The zero point as a nibble would be 1.5 of 67 bytes a group less; the

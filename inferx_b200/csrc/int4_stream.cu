@@ -34,33 +34,28 @@ __device__ __forceinline__ void i4s_mma(float* c, const unsigned* a, unsigned b0
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Eight activations of a row as fragments: [term][pair of k].
+// Four activations of a row as fragments: [term][pair of k].
 template <typename XT> struct I4Frag;
 template <> struct I4Frag<bf16> {
   static constexpr int TERMS = 1;
-  uint4 r;
+  uint2 r;
   __device__ __forceinline__ void load(const bf16* p, bool ok) {
-    r = ok ? *reinterpret_cast<const uint4*>(p) : make_uint4(0, 0, 0, 0);
+    r = ok ? *reinterpret_cast<const uint2*>(p) : make_uint2(0, 0);
   }
-  __device__ __forceinline__ void terms(unsigned (*b)[4]) const {
+  __device__ __forceinline__ void terms(unsigned (*b)[2]) const {
     b[0][0] = r.x;
     b[0][1] = r.y;
-    b[0][2] = r.z;
-    b[0][3] = r.w;
   }
 };
 template <> struct I4Frag<float> {
   static constexpr int TERMS = 3;
-  float4 lo, hi;
+  float4 r;
   __device__ __forceinline__ void load(const float* p, bool ok) {
-    lo = ok ? *reinterpret_cast<const float4*>(p) : make_float4(0.f, 0.f, 0.f, 0.f);
-    hi = ok ? *reinterpret_cast<const float4*>(p + 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+    r = ok ? *reinterpret_cast<const float4*>(p) : make_float4(0.f, 0.f, 0.f, 0.f);
   }
-  __device__ __forceinline__ void terms(unsigned (*b)[4]) const {
-    i4_terms2(lo.x, lo.y, b[0][0], b[1][0], b[2][0]);
-    i4_terms2(lo.z, lo.w, b[0][1], b[1][1], b[2][1]);
-    i4_terms2(hi.x, hi.y, b[0][2], b[1][2], b[2][2]);
-    i4_terms2(hi.z, hi.w, b[0][3], b[1][3], b[2][3]);
+  __device__ __forceinline__ void terms(unsigned (*b)[2]) const {
+    i4_terms2(r.x, r.y, b[0][0], b[1][0], b[2][0]);
+    i4_terms2(r.z, r.w, b[0][1], b[1][1], b[2][1]);
   }
 };
 
@@ -101,7 +96,7 @@ int4_stream_kernel(const XT* __restrict__ x, const int* __restrict__ rows,
                    int M_single, int N, int K, int strips, int chunks, int ksplit,
                    int offsets_settled) {
   typedef I4SCfg<NT, GROUP, S> C;
-  constexpr int NG = 128 / GROUP, PER = GROUP / 32;
+  constexpr int NG = 128 / GROUP, PER = GROUP / 16;
   constexpr int TERMS = I4Frag<XT>::TERMS, ACCS = TERMS == 3 ? 2 : 1;
   static_assert(!DUAL || S == 2, "a gate strip and its up strip");
   extern __shared__ __align__(16) unsigned char smem[];
@@ -171,7 +166,7 @@ int4_stream_kernel(const XT* __restrict__ x, const int* __restrict__ rows,
       const int r = r0 + i * 8 + g;
       xok[i] = r < hi;
       const size_t src = xok[i] ? (rows ? (size_t)rows[r] : (size_t)r) : 0;
-      xrow[i] = x + src * K + t * 8;
+      xrow[i] = x + src * K + t * 4;
     }
     float tot[S][NT][4];
 #pragma unroll
@@ -184,14 +179,14 @@ int4_stream_kernel(const XT* __restrict__ x, const int* __restrict__ rows,
       __syncwarp();                                // the previous pass has read its parameters
       for (int i = 0; i < C::R - 1; ++i) fetch(i);
     }
-    I4Frag<XT> f[4][NT], f_next[4][NT];
+    I4Frag<XT> f[8][NT], f_next[8][NT];
     auto fetch_x = [&](int i) {
       const int k0 = (ks + i * ksplit) * I4_CHUNK_K;
 #pragma unroll
-      for (int b = 0; b < 4; ++b)
+      for (int b = 0; b < 8; ++b)
 #pragma unroll
         for (int j = 0; j < NT; ++j)
-          f_next[b][j].load(xrow[j] + k0 + b * 32, xok[j] && i < n && k0 + b * 32 + t * 8 < K);
+          f_next[b][j].load(xrow[j] + k0 + b * 16, xok[j] && i < n && k0 + b * 16 + t * 4 < K);
     };
     fetch_x(0);
     for (int i = 0; i < n; ++i) {
@@ -199,7 +194,7 @@ int4_stream_kernel(const XT* __restrict__ x, const int* __restrict__ rows,
       __syncwarp();            // parameters were copied by other lanes; the last chunk's are read
       fetch(i + C::R - 1);
 #pragma unroll
-      for (int b = 0; b < 4; ++b)
+      for (int b = 0; b < 8; ++b)
 #pragma unroll
         for (int j = 0; j < NT; ++j) f[b][j] = f_next[b][j];
       fetch_x(i + 1);
@@ -219,7 +214,7 @@ int4_stream_kernel(const XT* __restrict__ x, const int* __restrict__ rows,
       }
       float acc[ACCS][S][NT][4];
 #pragma unroll
-      for (int b = 0; b < 4; ++b) {
+      for (int b = 0; b < 8; ++b) {
         if (b % PER == 0) {
 #pragma unroll
           for (int a = 0; a < ACCS; ++a)
@@ -230,32 +225,26 @@ int4_stream_kernel(const XT* __restrict__ x, const int* __restrict__ rows,
 #pragma unroll
                 for (int q = 0; q < 4; ++q) acc[a][s][j][q] = 0.f;
         }
-        unsigned a[S][2][4];
+        unsigned a[S][4];
 #pragma unroll
         for (int s = 0; s < S; ++s) {
-          const uint4 v = w[s][b >> 1];
-          const unsigned word[2] = {(b & 1) ? v.z : v.x, (b & 1) ? v.w : v.y};
+          const uint4 v = w[s][b >> 2];
+          const unsigned word = (b & 3) == 0 ? v.x : (b & 3) == 1 ? v.y : (b & 3) == 2 ? v.z : v.w;
           const unsigned sa = i4_sub(pa[s][b / PER]), sb = i4_sub(pb[s][b / PER]);
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            a[s][j][0] = i4_pair(word[j], 0, sa);
-            a[s][j][1] = i4_pair(word[j], 1, sb);
-            a[s][j][2] = i4_pair(word[j], 2, sa);
-            a[s][j][3] = i4_pair(word[j], 3, sb);
-          }
+          a[s][0] = i4_pair(word, 0, sa);
+          a[s][1] = i4_pair(word, 1, sb);
+          a[s][2] = i4_pair(word, 2, sa);
+          a[s][3] = i4_pair(word, 3, sb);
         }
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-          unsigned xb[TERMS][4];
+          unsigned xb[TERMS][2];
           f[b][j].terms(xb);
 #pragma unroll
           for (int m = TERMS - 1; m >= 0; --m)
 #pragma unroll
-            for (int s = 0; s < S; ++s) {
-              float* sum = acc[m > 0 ? ACCS - 1 : 0][s][j];
-              i4s_mma(sum, a[s][0], xb[m][0], xb[m][1]);
-              i4s_mma(sum, a[s][1], xb[m][2], xb[m][3]);
-            }
+            for (int s = 0; s < S; ++s)
+              i4s_mma(acc[m > 0 ? ACCS - 1 : 0][s][j], a[s], xb[m][0], xb[m][1]);
         }
         if (b % PER == PER - 1) {
 #pragma unroll

@@ -7,28 +7,29 @@
 // `a` holds bfloat16 rows grouped by expert (offsets), or the rows of a single matrix; fp32 rows come
 // as three planes of bfloat16 terms that are multiplied into the same sums.
 //
-// The weights are the M side of tcgen05.mma and the rows the N side.  Two SMs work on one item
-// (cta_group::2): 256 weight rows (DUAL: 128 gate rows and the up rows of the same columns) for a tile
-// of up to BT rows of one expert, over all of K or one of `splits` runs of it.  A block holds 128 of the
-// weight rows and half of the tile's rows, so each of the two halves is brought once.  Pairs are
-// persistent and take items round robin.  Roles of a block's twenty warps, a chunk of 128 k at a time:
+// The weights are the M side of tcgen05.mma, read from tensor memory, and the rows the N side, read from
+// shared memory.  Two SMs work on one item (cta_group::2): 256 weight rows (DUAL: 128 gate rows and the
+// up rows of the same columns) for a tile of up to BT rows of one expert, over all of K or one of
+// `splits` runs of it.  A block holds 128 of the weight rows and half of the tile's rows, so each of the
+// two halves is brought once.  Pairs are persistent and take items round robin.  Roles of a block's
+// warps, a chunk of 128 k at a time:
 //   0      brings the rows into a ring of stages (TMA, 128-byte swizzle);
 //   1      the first block's issues the MMAs for both, a group of k into one of two accumulators in
 //          tensor memory; the second block's tells the first that its own operands are there;
 //   2      brings the codes and parameters of the block's eight strips (one bulk copy, DUAL two);
-//   4-11   take each finished group's sums out of tensor memory, a weight row a lane, and add scale *
-//          sum to fp32 registers;
-//          Rows of a DUAL item lie as 16 gate rows, the 16 up rows of the same columns, and so on, so
-//          that a column's two sums are sixteen lanes of one warp apart;
-//   12-19  unpack a strip each: a lane's 16 bytes of codes are eight neighbouring k of two rows, twice; less their
-//          zero points they are whole numbers, written as a swizzled operand tile.
+//   4-11   take each finished group's sums out of tensor memory, a weight row a lane, add scale * sum to
+//          fp32 registers, and leave an item's results in shared memory;
+//   12-19  unpack a strip each: a lane's sixteen bytes of codes, less their zero points, are whole numbers
+//          that lie in registers as tensor memory wants them (16 rows by 256 bits);
+//   20-23  finish and store the results of an item while the next one is under way.
+// Rows of a DUAL item lie as 16 gate rows, the 16 up rows of the same columns, and so on.
 // So the operands of the tensor cores are exact (a code less its zero point has five bits), the sums of
 // a group are the tensor cores' fp32, and a group's scale multiplies in fp32: no weight is rounded to
 // bfloat16.
 //
 // Columns past the tile and weight rows past N are computed on whatever is there and never stored.
 // Every wait on an mbarrier is bounded: the waiter records a code in `status` (51 and 54 copies, 52
-// MMAs, 53 unpacking, 55 sums), raises a flag that ends its block's other roles, and the pair meets at
+// MMAs, 53 unpacking, 55 sums, 56 results), raises a flag that ends its block's other roles, and the pair meets at
 // its end, where tensor memory is freed.
 #include <type_traits>
 
@@ -36,22 +37,22 @@
 #include "tcgen05_common.cuh"
 #include "tma_common.cuh"
 
-#define I4T_THREADS 640
-#define I4T_TILE (128 * 64 * 2)           // 64 k of a block's weight rows, unpacked
+#define I4T_THREADS 768
 #define I4T_MAX_EXPERTS 1024              // the prefix of tiles lives in shared memory
 #define I4T_NAP 20000                     // ns
 #define I4T_WAIT_CLOCKS 4000000000LL      // about two seconds
 #define I4T_DONE 4                        // barriers of finished chunks
 
 enum {
-  I4T_ERR_COPY = 51, I4T_ERR_MMA = 52, I4T_ERR_UNPACK = 53, I4T_ERR_CODES = 54, I4T_ERR_SUM = 55
+  I4T_ERR_COPY = 51, I4T_ERR_MMA = 52, I4T_ERR_UNPACK = 53, I4T_ERR_CODES = 54, I4T_ERR_SUM = 55,
+  I4T_ERR_STORE = 56
 };
 
 struct I4TArgs {
   const int* offsets;       // null: one matrix with `rows` rows
   const unsigned* data;
   void* out;
-  float* part;              // splits > 1, or an activation: [splits][rows][columns of both halves] sums
+  float* part;              // splits > 1: [splits][rows][columns of both halves] sums
   int wide;                 // fp32 results, otherwise bfloat16
   const float* row_scale;
   int plain;
@@ -71,17 +72,18 @@ template <int TERMS, bool DUAL, int BT, int GROUP> struct I4TCfg {
   static constexpr int X_STAGE = TERMS * 2 * X_TILE;
   static constexpr int BOX = BT / 4;                           // rows of a TMA box
   static constexpr int C_BYTES = i4_block_words(GROUP) * 4;    // a strip's codes and parameters
-  static constexpr int X_RING = TERMS == 3 ? 2 : BT == 256 ? 3 : 4;
-  static constexpr int A_RING = TERMS == 3 ? 2 : 3;
-  static constexpr int C_RING = BT == 128 ? 4 : 2;
+  static constexpr int X_RING = TERMS == 3 ? 2 : 4;
+  static constexpr int C_RING = BT == 128 ? 4 : GROUP == 128 ? 3 : 2;
+  // Tensor memory: two accumulators of BT columns, and operand stages of 128 k (64 columns)
+  static constexpr int A_RING = (512 - 2 * BT) / 64;
   // Scales are written once the MMAs of A_RING chunks before have run, and those had waited for the
   // sums of two chunks before them to be taken: a slot is read by then.
   static constexpr int S_RING = A_RING + 2;
-  static constexpr int SMEM = X_RING * X_STAGE + A_RING * 2 * I4T_TILE + C_RING * 8 * C_BYTES +
+  static constexpr int SMEM = X_RING * X_STAGE + BT * 128 * 4 + C_RING * 8 * C_BYTES +
                               S_RING * 128 * (128 / GROUP) * 2 + 1024;
   static_assert(SMEM + 4608 <= 227 * 1024, "shared memory");
   static_assert(X_RING <= I4T_DONE && A_RING <= I4T_DONE, "a stage's last use is still to be seen");
-  static constexpr unsigned TMEM_COLS = 2 * BT;
+  static_assert(BT % 64 == 0 && 2 * BT + 64 * A_RING <= 512, "tensor memory");
   static constexpr int F = DUAL ? 128 : 256;                   // output columns of an item
 };
 
@@ -123,6 +125,40 @@ __device__ __forceinline__ bool i4t_wait(unsigned long long* bar, unsigned parit
   }
   return false;
 }
+// The pair's MMA with the weights in tensor memory (each block's rows in its own).
+__device__ __forceinline__ void i4t_mma(unsigned d, unsigned a, unsigned long long bdesc,
+                                        unsigned idesc, unsigned accum) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(bdesc), "r"(idesc), "r"(accum)
+      : "memory");
+}
+// Sixteen rows by 64 k of an operand: four registers a lane for every sixteen k.
+__device__ __forceinline__ void i4t_put(unsigned taddr, const unsigned* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.16x256b.x4.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+      "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
+}
+// sixteen columns of this thread's lane
+__device__ __forceinline__ void i4t_ld16(unsigned taddr, float* v) {
+  unsigned r[16];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
 // two fp32 numbers as one 64-bit register, and a * b + c on both
 __device__ __forceinline__ unsigned long long i4t_pack(float a, float b) {
   unsigned long long r;
@@ -146,16 +182,17 @@ template <int NG> __device__ __forceinline__ void i4t_scales(unsigned short* to,
         make_uint2(__byte_perm(v[0], v[NG > 1 ? 1 : 0], 0x5410),
                    __byte_perm(v[NG > 2 ? 2 : 0], v[NG - 1], 0x5410));
 }
-// Out of line: an epilogue that holds it unrolled runs from a cold instruction cache.
-__device__ __noinline__ float i4t_silu_wide(float a, float u) { return a / (1.0f + expf(-a)) * u; }
-
 // sum += scale * (32 columns of this thread's lane)
 __device__ __forceinline__ void i4t_add(unsigned long long* sum, unsigned long long scale,
                                         unsigned taddr) {
-  float v[32];
-  tc_ld32(taddr, v);
 #pragma unroll
-  for (int j = 0; j < 16; ++j) i4t_fma2(sum[j], scale, i4t_pack(v[2 * j], v[2 * j + 1]));
+  for (int h = 0; h < 2; ++h) {
+    float v[16];
+    i4t_ld16(taddr + 16 * h, v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      i4t_fma2(sum[8 * h + j], scale, i4t_pack(v[2 * j], v[2 * j + 1]));
+  }
 }
 
 template <int BT>
@@ -170,8 +207,8 @@ int4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
   extern __shared__ unsigned char smem_raw[];
   unsigned char* xs =
       reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  unsigned char* as = xs + C::X_RING * C::X_STAGE;
-  unsigned char* cs = as + C::A_RING * 2 * I4T_TILE;
+  float* stage = reinterpret_cast<float*>(xs + C::X_RING * C::X_STAGE);   // [row of the tile][128]
+  unsigned char* cs = reinterpret_cast<unsigned char*>(stage + BT * 128);
   unsigned short* scales = reinterpret_cast<unsigned short*>(cs + C::C_RING * 8 * C::C_BYTES);
   // A group may be multiplied: on a chunk's first group the block's operands are there (eight unpacking
   // warps and the rows' bytes), an accumulator's sums are taken (eight warps), and, in the first block,
@@ -182,6 +219,7 @@ int4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
   __shared__ __align__(8) unsigned long long done[I4T_DONE];     // a chunk's MMAs have run
   __shared__ __align__(8) unsigned long long full_s[C::S_RING];  // a chunk's scales are there
   __shared__ __align__(8) unsigned long long acc_full[2];
+  __shared__ __align__(8) unsigned long long stage_full, stage_empty;
   __shared__ unsigned tmem_holder;
   __shared__ int abort_flag;
   __shared__ int tile_start[I4T_MAX_EXPERTS + 1];
@@ -220,11 +258,13 @@ int4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
     for (int s = 0; s < I4T_DONE; ++s) mbar_init(&done[s], 1);
     for (int s = 0; s < C::S_RING; ++s) mbar_init(&full_s[s], 8);
     for (int b = 0; b < 2; ++b) mbar_init(&acc_full[b], 1);
+    mbar_init(&stage_full, 8);
+    mbar_init(&stage_empty, 4);
     abort_flag = 0;
     mbar_init_fence();
     fence_proxy_async();
   }
-  if (warp == 1) tc_alloc<true>(&tmem_holder, C::TMEM_COLS);
+  if (warp == 1) tc_alloc<true>(&tmem_holder, 512);
   tc_fence_before();
   __syncthreads();
   tc_cluster_sync();
@@ -271,8 +311,8 @@ int4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
     return (bool)__all_sync(0xffffffffu, i4t_wait(bar, parity, abortp));
   };
 
-  // Registers go from the roles that need few to the warps that hold up to 128 sums a lane (640
-  // threads at 96: 128 x 32 + 256 x 168 + 256 x 56).
+  // Registers go from the roles that need few to the warps that hold up to 96 sums a lane (768
+  // threads at 80: 128 x 32 + 256 x 136 + 256 x 56 + 128 x 56).
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");
     if (warp == 0) {
@@ -325,30 +365,30 @@ int4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
                                ((unsigned)(((it.n + 31) & ~31) >> 3) << 17) | (16u << 24);
         for (int c = it.c0; c < it.c1 && ok; ++c, ++n) {
           const int slot = n % I4T_DONE;
-          const unsigned long long ad = umma_desc(as + (n % C::A_RING) * 2 * I4T_TILE);
+          const unsigned ad = tmem_base + 2 * BT + (n % C::A_RING) * 64;
           const unsigned long long xd = umma_desc(xs + (n % C::X_RING) * C::X_STAGE);
           for (int q = 0; q < NG; ++q, ++group) {
             ok = wait(&go[slot][q], n / I4T_DONE & 1);
             if (!ok) break;
+            tc_fence_after();
             if (rank != 0) {
+              tc_fence_before();
               if (lane == 0) i4t_arrive_at(first_block + (slot * NG + q) * 8);
               __syncwarp();
               continue;
             }
-            tc_fence_after();
             const int buf = group & 1;
             const unsigned sums = tmem_base + buf * BT;
             if (lane == 0) {
 #pragma unroll
               for (int i = 0; i < GROUP / 16; ++i) {
-                // sixteens of k into the chunk; 32 bytes each inside a tile's swizzled rows
+                // sixteens of k into the chunk: eight columns of weights, 32 bytes of a row
                 const int at = q * (GROUP / 16) + i;
-                const unsigned long long a = ad + (at >> 2) * (I4T_TILE >> 4) + (at & 3) * 2;
 #pragma unroll
                 for (int t = TERMS - 1; t >= 0; --t)           // small terms first
-                  tc_mma_pair(sums, a,
-                              xd + (t * 2 + (at >> 2)) * (C::X_TILE >> 4) + (at & 3) * 2, idesc,
-                              i == 0 && t == TERMS - 1 ? 0u : 1u);
+                  i4t_mma(sums, ad + at * 8,
+                          xd + (t * 2 + (at >> 2)) * (C::X_TILE >> 4) + (at & 3) * 2, idesc,
+                          i == 0 && t == TERMS - 1 ? 0u : 1u);
               }
               if (NG > 1) tc_commit_pair(&acc_full[buf]);
               if (q == NG - 1) tc_commit_pair(&done[slot]);
@@ -393,11 +433,96 @@ int4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
           mbar_drain(&full_c[f % C::C_RING], f / C::C_RING & 1);
       }
     }
+  } else if (warp >= 20) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    // Units of eight neighbouring columns of one row: sixteen a row (DUAL: eight), so 256 threads'
+    // worth a pass; consecutive threads take consecutive units.
+    constexpr int COLS = F / 2, UNITS = COLS / 8;
+    const int thread = threadIdx.x - 20 * 32;
+    const int unit = thread % UNITS;
+    const int at = DUAL ? (unit >> 1) * 32 + (unit & 1) * 8 : unit * 8;      // its first entry of a row
+    const bool whole = p.N % 8 == 0 && ((uintptr_t)p.out & 15) == 0;
+    int k = 0;                               // items so far
+    bool ok = true;
+    for (int w = first; w < n_items && ok; w += step) {
+      const I4TItem it = item_of(w);
+      if (it.n <= 0) continue;
+      ok = wait(&stage_full, k & 1);
+      if (!ok) break;
+      const int f = it.f0 + rank * COLS + unit * 8;
+      const int cols = min(8, p.N - f);
+      if (cols > 0)
+        for (int r = thread / UNITS; r < it.n; r += 128 / UNITS) {
+          float v[8], u[8];
+          *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(stage + r * 128 + at);
+          *reinterpret_cast<float4*>(v + 4) =
+              *reinterpret_cast<const float4*>(stage + r * 128 + at + 4);
+          if (DUAL) {
+            *reinterpret_cast<float4*>(u) = *reinterpret_cast<const float4*>(stage + r * 128 + at + 16);
+            *reinterpret_cast<float4*>(u + 4) =
+                *reinterpret_cast<const float4*>(stage + r * 128 + at + 20);
+          }
+          const size_t row = (size_t)(it.m0 + r);
+          if (p.part) {                      // sums of a run of K: the halves' columns beside each other
+            const size_t width = DUAL ? 2 * (size_t)p.N : (size_t)p.N;
+            float* o = p.part + ((size_t)it.z * p.rows + row) * width + f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              if (i < cols) {
+                o[i] = v[i];
+                if (DUAL) o[p.N + i] = u[i];
+              }
+            continue;
+          }
+          if (DUAL) {
+            const float s = p.row_scale ? p.row_scale[row] : 1.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const float a = v[i] * s;
+              v[i] = p.wide ? a / (1.0f + expf(-a)) * (u[i] * s)
+                            : __fdividef(a, 1.0f + __expf(-a)) * (u[i] * s);
+            }
+          } else if (p.plain) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              v[i] = p.wide ? ix_act<float>(v[i], p.plain) : ix_act<bf16>(v[i], p.plain);
+          }
+          const size_t to = row * p.N + f;
+          if (p.wide) {
+            float* o = (float*)p.out + to;
+            if (whole) {
+              *reinterpret_cast<float4*>(o) = *reinterpret_cast<float4*>(v);
+              *reinterpret_cast<float4*>(o + 4) = *reinterpret_cast<float4*>(v + 4);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                if (i < cols) o[i] = v[i];
+            }
+          } else {
+            bf16* o = (bf16*)p.out + to;
+            if (whole) {
+              __nv_bfloat162 h[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+              *reinterpret_cast<uint4*>(o) = *reinterpret_cast<uint4*>(h);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                if (i < cols) o[i] = __float2bfloat16_rn(v[i]);
+            }
+          }
+        }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&stage_empty);
+      ++k;
+    }
+    if (!ok && lane == 0 && !*abortp) { atomicExch(p.status, I4T_ERR_STORE); *abortp = 1; }
   } else if (warp >= 12) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    const int unpacker = warp - 12;          // its strip (DUAL: gate strips are 0, 2, 4, 6)
+    // its strip: one that the warp's lanes of tensor memory hold
+    const int unpacker = 2 * (warp & 3) + ((warp - 12) >> 2);
     const int g = lane >> 2, t = lane & 3;
-    const bool odd = g & 1;
+    const unsigned to = tmem_base + 2 * BT + ((unsigned)(unpacker * 16) << 16);
     // (DUAL: four gate strips were copied, then four up strips)
     const int from = DUAL ? (unpacker & 1) * 4 + (unpacker >> 1) : unpacker;
     int n = 0;
@@ -432,34 +557,24 @@ int4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
           i4t_scales<NG>(to, pa);
           i4t_scales<NG>(to + 8 * NG, pb);
         }
+        tc_fence_after();
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          unsigned char* at = as + (sa * 2 + h) * I4T_TILE + unpacker * 2048 + g * 128;
+          const unsigned word[4] = {code[h].x, code[h].y, code[h].z, code[h].w};
+          unsigned v[16];
 #pragma unroll
-          for (int run = 0; run < 2; ++run) {
-            // lanes of odd rows take the two runs of eight k the other way round, so that the
-            // eight lanes of a store phase meet all banks
-            const bool second = (run == 1) != odd;
-            const unsigned w0 = second ? code[h].z : code[h].x;
-            const unsigned w1 = second ? code[h].w : code[h].y;
-            unsigned sa2, sb2;
-            if (GROUP == 32) {
-              sa2 = i4_sub(second ? pa[(2 * h + 1) % NG] : pa[2 * h % NG]);
-              sb2 = i4_sub(second ? pb[(2 * h + 1) % NG] : pb[2 * h % NG]);
-            } else {
-              sa2 = i4_sub(pa[GROUP == 64 ? h % NG : 0]);
-              sb2 = i4_sub(pb[GROUP == 64 ? h % NG : 0]);
-            }
-            const int where = (((second ? 4 : 0) + t) ^ g) * 16;
-            *reinterpret_cast<uint4*>(at + where) =
-                make_uint4(i4_pair(w0, 0, sa2), i4_pair(w0, 2, sa2), i4_pair(w1, 0, sa2),
-                           i4_pair(w1, 2, sa2));
-            *reinterpret_cast<uint4*>(at + 1024 + where) =
-                make_uint4(i4_pair(w0, 1, sb2), i4_pair(w0, 3, sb2), i4_pair(w1, 1, sb2),
-                           i4_pair(w1, 3, sb2));
+          for (int j = 0; j < 4; ++j) {
+            const int group = (h * 4 + j) * 16 / GROUP;
+            const unsigned sa2 = i4_sub(pa[group]), sb2 = i4_sub(pb[group]);
+            v[4 * j] = i4_pair(word[j], 0, sa2);
+            v[4 * j + 1] = i4_pair(word[j], 2, sa2);
+            v[4 * j + 2] = i4_pair(word[j], 1, sb2);
+            v[4 * j + 3] = i4_pair(word[j], 3, sb2);
           }
+          i4t_put(to + sa * 64 + h * 32, v);
         }
-        fence_proxy_async();
+        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+        tc_fence_before();
         __syncwarp();
         if (lane == 0) {
           mbar_arrive(&go[n % I4T_DONE][0]);
@@ -469,10 +584,10 @@ int4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
     }
     if (!ok && lane == 0 && !*abortp) { atomicExch(p.status, I4T_ERR_UNPACK); *abortp = 1; }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 136;");
     const int quarter = warp & 3, half = (warp - 4) >> 2;  // lanes of tensor memory; every second 32 rows
     const unsigned lanes = tmem_base + ((unsigned)(quarter * 32) << 16);
-    int n = 0, group = 0;
+    int n = 0, group = 0, items = 0;
     bool ok = true;
     // group g's accumulator is free
     auto free_for = [&](int g) {
@@ -521,102 +636,25 @@ int4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
         }
       }
       if (!ok) break;
-      // -- a lane holds one weight row for 32 rows at a time: 64- or 128-byte stores of a warp
-      const int f_own = it.f0 + rank * (F / 2);
-      if (p.part) {
-        // sums of a run of K: the halves' columns beside each other
-        const int f = DUAL ? f_own + quarter * 16 + (lane & 15) : f_own + quarter * 32 + lane;
-        const size_t width = DUAL ? 2 * (size_t)p.N : (size_t)p.N;
-        float* o = p.part + ((size_t)it.z * p.rows + it.m0) * width +
-                   (DUAL && lane >= 16 ? p.N : 0) + f;
+      // the item's results, a weight row a lane, to the warps that store them
+      ok = wait(&stage_empty, (items & 1) ^ 1);
+      if (!ok) break;
+      float* mine = stage + quarter * 32 + lane;
 #pragma unroll
-        for (int i = 0; i < BT / 64; ++i) {
-          const int col = 64 * i + 32 * half;
-          const int n_here = f < p.N ? it.n - col : 0;
+      for (int i = 0; i < BT / 64; ++i) {
+        const int col = 64 * i + 32 * half;
+        if (col >= it.n) continue;
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            float a, b;
-            i4t_unpack(sum[i][j], a, b);
-            if (2 * j < n_here) o[(size_t)(col + 2 * j) * width] = a;
-            if (2 * j + 1 < n_here) o[(size_t)(col + 2 * j + 1) * width] = b;
-          }
+        for (int j = 0; j < 16; ++j) {
+          float a, b;
+          i4t_unpack(sum[i][j], a, b);
+          mine[(col + 2 * j) * 128] = a;
+          mine[(col + 2 * j + 1) * 128] = b;
         }
-      } else if (DUAL) {
-        // of two neighbouring rows the lanes with the gate's sums take the first, those with the
-        // up sums the second: each gets the other sum of its row
-        const bool up = lane >= 16;
-        const int f = f_own + quarter * 16 + (lane & 15);
-        auto finish = [&](auto wide, auto scaled) {
-#pragma unroll
-          for (int i = 0; i < BT / 64; ++i) {
-            const int col = 64 * i + 32 * half + (up ? 1 : 0);
-            if (64 * i + 32 * half >= it.n) continue;
-            const int n_here = f < p.N ? it.n - col : 0;
-            const size_t at = (size_t)(it.m0 + col) * p.N + f;
-            const size_t two = 2 * (size_t)p.N;
-            float* o = (float*)p.out + at;
-            bf16* ob = (bf16*)p.out + at;
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              float first_row, second_row;
-              i4t_unpack(sum[i][j], first_row, second_row);
-              const float got = __shfl_xor_sync(0xffffffffu, up ? first_row : second_row, 16);
-              float a = up ? got : first_row, u = up ? second_row : got;
-              if (scaled.value) {
-                const float s = 2 * j < n_here ? p.row_scale[it.m0 + col + 2 * j] : 0.f;
-                a *= s;
-                u *= s;
-              }
-              if (wide.value) {
-                const float y = i4t_silu_wide(a, u);
-                if (2 * j < n_here) *o = y;
-                o += two;
-              } else {
-                const float y = __fdividef(a, 1.0f + __expf(-a)) * u;
-                if (2 * j < n_here) *ob = __float2bfloat16_rn(y);
-                ob += two;
-              }
-            }
-          }
-        };
-        if (p.wide) {
-          if (p.row_scale) finish(std::true_type(), std::true_type());
-          else finish(std::true_type(), std::false_type());
-        } else {
-          if (p.row_scale) finish(std::false_type(), std::true_type());
-          else finish(std::false_type(), std::false_type());
-        }
-      } else {
-        const int f = f_own + quarter * 32 + lane;
-        auto finish = [&](auto wide) {
-#pragma unroll
-          for (int i = 0; i < BT / 64; ++i) {
-            const int col = 64 * i + 32 * half;
-            if (col >= it.n) continue;
-            const int n_here = f < p.N ? it.n - col : 0;
-            const size_t at = (size_t)(it.m0 + col) * p.N + f;
-            float* o = (float*)p.out + at;
-            bf16* ob = (bf16*)p.out + at;
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              float y[2];
-              i4t_unpack(sum[i][j], y[0], y[1]);
-#pragma unroll
-              for (int k = 0; k < 2; ++k) {
-                if (wide.value) {
-                  if (2 * j + k < n_here) *o = y[k];
-                  o += p.N;
-                } else {
-                  if (2 * j + k < n_here) *ob = __float2bfloat16_rn(y[k]);
-                  ob += p.N;
-                }
-              }
-            }
-          }
-        };
-        if (p.wide) finish(std::true_type());
-        else finish(std::false_type());
       }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&stage_full);
+      ++items;
     }
     if (!ok && lane == 0 && !*abortp) { atomicExch(p.status, I4T_ERR_SUM); *abortp = 1; }
   }
@@ -624,7 +662,7 @@ int4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
   __syncthreads();
   // neither block ends while the other can still reach its barriers, tiles or accumulators
   tc_cluster_sync();
-  if (warp == 1) tc_dealloc<true>(tmem_base, C::TMEM_COLS);
+  if (warp == 1) tc_dealloc<true>(tmem_base, 512);
 }
 
 // The runs' sums in ascending order, and what follows them.
@@ -701,13 +739,13 @@ static I4TPlan i4t_plan(int rows, int N, int Kp, int E, bool grouped, bool dual,
   if (grouped) {
     // the mean rows of an expert, and some for imbalance
     plan.large = terms == 1 && 1.15 * rows / E > 128.0;
-    plan.tile_rows = plan.large ? 256 : 128;
+    plan.tile_rows = plan.large ? 192 : 128;
     const long long tiles = (rows < E ? rows : E) * f_tiles;
     while (rows <= 4096 && plan.splits < 16 && tiles * plan.splits * 2 <= pairs && chunks / (plan.splits * 2) >= 2)
       plan.splits *= 2;
     return plan;
   }
-  const int most = rows > 128 && terms == 1 ? 256 : 128;
+  const int most = rows > 128 && terms == 1 ? 192 : 128;
   const int cuts0 = (rows + most - 1) / most;
   for (int cuts = cuts0; cuts <= cuts0 + 8; ++cuts) {
     const int per = ((rows + cuts - 1) / cuts + 31) & ~31;
@@ -730,11 +768,10 @@ static I4TPlan i4t_plan(int rows, int N, int Kp, int E, bool grouped, bool dual,
 }
 
 // fp32 entries of scratch that a call of these sizes wants (0: none)
-IX_API long long ix_int4_tc_scratch(int rows, int N, int Kp, int E, int grouped, int dual, int terms,
-                                    int plain) {
+IX_API long long ix_int4_tc_scratch(int rows, int N, int Kp, int E, int grouped, int dual, int terms) {
   if (rows <= 0 || N <= 0 || Kp <= 0 || E <= 0) return 0;
   const I4TPlan plan = i4t_plan(rows, N, Kp, E, grouped != 0, dual != 0, terms);
-  return plan.splits > 1 || plain ? (long long)plan.splits * rows * N * (dual ? 2 : 1) : 0;
+  return plan.splits > 1 ? (long long)plan.splits * rows * N * (dual ? 2 : 1) : 0;
 }
 
 // x: [rows, Kp] bf16, or [3, rows, Kp] terms of fp32 rows; Kp a multiple of 8 that ends in the last
@@ -751,7 +788,7 @@ IX_API int ix_int4_tc(const void* x, int terms, const int* offsets, const void* 
   if (((uintptr_t)x | (uintptr_t)data) & 15) return IX_ERR_ALIGN;
   if (3LL * rows > 0x7fffffffLL || N > 0x3fffff00) return IX_ERR_SIZE;
   const I4TPlan plan = i4t_plan(rows, N, Kp, E, offsets != nullptr, dual != 0, terms);
-  if (plan.splits > 1 || plain) {
+  if (plan.splits > 1) {
     if (part == nullptr) return IX_ERR_SIZE;
   } else {
     part = nullptr;
@@ -770,10 +807,10 @@ IX_API int ix_int4_tc(const void* x, int terms, const int* offsets, const void* 
   } while (0)
   if (terms == 1) {
     if (dual) {
-      if (plan.large) I4T_BT(1, true, 256);
+      if (plan.large) I4T_BT(1, true, 192);
       I4T_BT(1, true, 128);
     }
-    if (plan.large) I4T_BT(1, false, 256);
+    if (plan.large) I4T_BT(1, false, 192);
     I4T_BT(1, false, 128);
   }
   if (terms == 3) {

@@ -53,36 +53,32 @@ __device__ __forceinline__ size_t i4_block(const I4Place& p, int strips, int chu
   return ((size_t)p.m * chunks + p.chunk) * strips + p.strip;
 }
 
-// The 32 entries of a row that a lane of `t` holds of a chunk, from `src` (the row, or null: zeros).
+// The 32 entries of a row that a lane of `t` holds of a chunk, four of every sixteen, from `src` (the
+// row, or null: zeros).
 template <typename T>
 __device__ __forceinline__ void i4_row_entries(const T* src, int k0, int K, int t, bool vec,
                                                float* v) {
 #pragma unroll
-  for (int b = 0; b < 4; ++b) {                    // blocks of 32 k
-    const int k = k0 + b * 32 + t * 8;
-    if (vec && src && k < K) {                     // K is a multiple of 8
+  for (int b = 0; b < 8; ++b) {                    // blocks of 16 k
+    const int k = k0 + b * 16 + t * 4;
+    if (vec && src && k < K) {                     // K is a multiple of 4
       if (sizeof(T) == 2) {
-        const uint4 r = *reinterpret_cast<const uint4*>(src + k);
-        const unsigned u[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          v[b * 8 + 2 * i] = __uint_as_float(u[i] << 16);
-          v[b * 8 + 2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
-        }
+        const uint2 r = *reinterpret_cast<const uint2*>(src + k);
+        v[b * 4] = __uint_as_float(r.x << 16);
+        v[b * 4 + 1] = __uint_as_float(r.x & 0xffff0000u);
+        v[b * 4 + 2] = __uint_as_float(r.y << 16);
+        v[b * 4 + 3] = __uint_as_float(r.y & 0xffff0000u);
       } else {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const float4 r = *reinterpret_cast<const float4*>(src + k + 4 * i);
-          v[b * 8 + 4 * i] = r.x;
-          v[b * 8 + 4 * i + 1] = r.y;
-          v[b * 8 + 4 * i + 2] = r.z;
-          v[b * 8 + 4 * i + 3] = r.w;
-        }
+        const float4 r = *reinterpret_cast<const float4*>(src + k);
+        v[b * 4] = r.x;
+        v[b * 4 + 1] = r.y;
+        v[b * 4 + 2] = r.z;
+        v[b * 4 + 3] = r.w;
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        v[b * 8 + i] = (src && k + i < K) ? to_f32<T>(src[k + i]) : 0.f;
+      for (int i = 0; i < 4; ++i)
+        v[b * 4 + i] = (src && k + i < K) ? to_f32<T>(src[k + i]) : 0.f;
     }
   }
 }
@@ -94,8 +90,8 @@ __device__ __forceinline__ void i4_store_words(unsigned* dst, int lane, const un
   for (int tile = 0; tile < 2; ++tile) {
     unsigned w[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {                  // word 2 h + j
-      const int at = tile * 16 + (i >> 1) * 8 + (i & 1) * 4;
+    for (int i = 0; i < 4; ++i) {
+      const int at = tile * 16 + i * 4;
       w[i] = (unsigned)ca[at] | ((unsigned)ca[at + 1] << 16) | ((unsigned)cb[at] << 4) |
              ((unsigned)cb[at + 1] << 20) | ((unsigned)ca[at + 2] << 8) |
              ((unsigned)ca[at + 3] << 24) | ((unsigned)cb[at + 2] << 12) |
@@ -183,18 +179,15 @@ i4_pack_kernel(const unsigned char* __restrict__ in, const bf16* __restrict__ sc
       const bf16 scale = there ? scales[r * groups + group] : __ushort_as_bfloat16(0);
       const int zero = there ? zeros[r * groups + group] & 15 : 0;
 #pragma unroll
-      for (int b = 0; b < PER; ++b) {
-        const int at = (n * PER + b) * 8, k = k0 + (n * PER + b) * 32 + t * 8;
-        if (vec && there && k < K) {               // K is a multiple of 8
-          const uint2 q = *reinterpret_cast<const uint2*>(in + r * K + k);
+      for (int b = 0; b < 2 * PER; ++b) {          // blocks of 16 k
+        const int at = (n * 2 * PER + b) * 4, k = k0 + (n * 2 * PER + b) * 16 + t * 4;
+        if (vec && there && k < K) {               // K is a multiple of 4
+          const unsigned q = *reinterpret_cast<const unsigned*>(in + r * K + k);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            code[side][at + i] = (q.x >> (8 * i)) & 15;
-            code[side][at + 4 + i] = (q.y >> (8 * i)) & 15;
-          }
+          for (int i = 0; i < 4; ++i) code[side][at + i] = (q >> (8 * i)) & 15;
         } else {
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
+          for (int i = 0; i < 4; ++i)
             code[side][at + i] = there && k + i < K ? in[r * K + k + i] & 15 : zero;
         }
       }
@@ -228,22 +221,20 @@ i4_unpack_kernel(const unsigned* __restrict__ data, unsigned char* __restrict__ 
     if (row >= rows) continue;
     const size_t r = (size_t)p.m * rows + row;
 #pragma unroll
-    for (int b = 0; b < 4; ++b) {
-      const int k = k0 + b * 32 + t * 8;
-      const uint4 q = w[b >> 1];
-      const unsigned lo = (b & 1) ? q.z : q.x, hi = (b & 1) ? q.w : q.y;
-      unsigned o[2];
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {                // four codes of a row out of a word
-        const unsigned u = (j ? hi : lo) >> (4 * side);
-        o[j] = (u & 15) | ((u >> 16 & 15) << 8) | ((u >> 8 & 15) << 16) | ((u >> 24 & 15) << 24);
-      }
+    for (int b = 0; b < 8; ++b) {
+      const int k = k0 + b * 16 + t * 4;
+      const uint4 q = w[b >> 2];
+      const unsigned u = ((b & 3) == 0 ? q.x : (b & 3) == 1 ? q.y : (b & 3) == 2 ? q.z : q.w) >>
+                         (4 * side);
+      // four codes of the row out of a word
+      const unsigned o = (u & 15) | ((u >> 16 & 15) << 8) | ((u >> 8 & 15) << 16) |
+                         ((u >> 24 & 15) << 24);
       if (vec && k < K) {
-        *reinterpret_cast<uint2*>(out + r * K + k) = make_uint2(o[0], o[1]);
+        *reinterpret_cast<unsigned*>(out + r * K + k) = o;
       } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (k + i < K) out[r * K + k + i] = (unsigned char)(o[i >> 2] >> (8 * (i & 3)));
+        for (int i = 0; i < 4; ++i)
+          if (k + i < K) out[r * K + k + i] = (unsigned char)(o >> (8 * i));
       }
     }
     for (int n = t; n < NG; n += 4) {
@@ -281,7 +272,7 @@ IX_API int ix_int4_quantize(const void* w, int dtype, void* data, long long matr
   unsigned grid;
   const int rc = i4_grid(matrices, rows, K, strips, chunks, grid);
   if (rc != IX_OK) return rc;
-  const int vec = K % 8 == 0 && ((uintptr_t)w & 15) == 0;
+  const int vec = K % 4 == 0 && ((uintptr_t)w & 15) == 0;
   IX_DISPATCH_DTYPE(dtype, T, {
     I4_GROUPS(G, i4_quantize_kernel<T, G><<<grid, I4_WARPS * 32, 0, stream>>>(
                      (const T*)w, (unsigned*)data, matrices, rows, K, strips,
@@ -298,7 +289,7 @@ IX_API int ix_int4_pack(const void* in, const void* scales, const void* zeros, v
   unsigned grid;
   const int rc = i4_grid(matrices, rows, K, strips, chunks, grid);
   if (rc != IX_OK) return rc;
-  const int vec = K % 8 == 0 && ((uintptr_t)in & 7) == 0;
+  const int vec = K % 4 == 0 && ((uintptr_t)in & 3) == 0;
   I4_GROUPS(G, i4_pack_kernel<G><<<grid, I4_WARPS * 32, 0, stream>>>(
                    (const unsigned char*)in, (const bf16*)scales, (const unsigned char*)zeros,
                    (unsigned*)data, matrices, rows, K, strips, chunks, vec));
@@ -312,7 +303,7 @@ IX_API int ix_int4_unpack(const void* data, void* out, void* scales,
   unsigned grid;
   const int rc = i4_grid(matrices, rows, K, strips, chunks, grid);
   if (rc != IX_OK) return rc;
-  const int vec = K % 8 == 0 && ((uintptr_t)out & 7) == 0;
+  const int vec = K % 4 == 0 && ((uintptr_t)out & 3) == 0;
   I4_GROUPS(G, i4_unpack_kernel<G><<<grid, I4_WARPS * 32, 0, stream>>>(
                    (const unsigned*)data, (unsigned char*)out, (bf16*)scales,
                    (unsigned char*)zeros, matrices, rows, K, strips, chunks, vec));

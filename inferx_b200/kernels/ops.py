@@ -1343,6 +1343,7 @@ _STATUS_ROLES = {
     41: "gemm_fp32_tc: a splitting warp", 42: "gemm_fp32_tc: the MMA issuer",
     51: "int4_tc: the copying warp", 52: "int4_tc: the MMA issuer", 53: "int4_tc: an unpacking warp",
     54: "int4_tc: the warp that copies codes", 55: "int4_tc: a warp that adds up",
+    56: "int4_tc: a warp that stores",
 }
 
 
@@ -1691,8 +1692,7 @@ def _int4_tc(what, x, rows, offsets, w, num_rows, out_dtype, row_scale=None, act
     lib = _lib()
     lib.ix_int4_tc_scratch.restype = ctypes.c_longlong
     need = lib.ix_int4_tc_scratch(num_rows, w.cols, x.shape[-1], w.experts,
-                                  0 if offsets is None else 1, w.halves - 1, terms,
-                                  _ACTIVATIONS[activation])
+                                  0 if offsets is None else 1, w.halves - 1, terms)
     part = torch.empty(need, dtype=torch.float32, device=x.device) if need else None
     _check(lib.ix_int4_tc(
         _ptr(x), terms, _ptr(offsets), _ptr(w.data), _ptr(out), _ptr(part),
