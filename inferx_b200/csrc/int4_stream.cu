@@ -11,13 +11,12 @@
 // Mapping: out^T = w . x^T with mma.sync.m16n8k16, sixteen weight rows the M side, eight activation
 // rows the N side.  A warp holds S strips of 16 weight rows (DUAL: a gate strip and the up strip of the
 // same columns) against 8 NT activation rows, so an activation fragment serves them all.  Blocks of
-// 128 k come by cp.async into a ring of the warp's own (nobody else reads it: no barrier in the loop),
-// R - 1 of them in flight; the next chunk's activations are loaded ahead into registers.  Each word of
-// codes becomes the A side of one mma by three shifts, four logic operations and four exact
-// subtractions, and the fp32 sums of a group are multiplied by the group's scale.  fp32 activations are
-// three bfloat16 terms, the two small ones summed apart from the first.  The warps of a block split K by
-// chunks and join their sums through shared memory in warp order, so a row's result does not depend on
-// which rows share its tile.
+// codes and the activations of the same 128 k come by cp.async into a ring of the warp's own (nobody
+// else reads it: no barrier in the loop), R - 1 chunks in flight.  Each word of codes becomes the A side
+// of one mma by three shifts, four logic operations and four exact subtractions, and the fp32 sums of a
+// group are multiplied by the group's scale.  fp32 activations are three bfloat16 terms, the two small
+// ones summed apart from the first.  The warps of a block split K by chunks and join their sums through
+// shared memory in warp order, so a row's result does not depend on which rows share its tile.
 #include "int4_format.cuh"
 
 #define I4S_THREADS 256
@@ -25,6 +24,11 @@
 
 __device__ __forceinline__ void i4s_copy16(unsigned to, const void* from) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+// the first `bytes` of 16, zeros behind them
+__device__ __forceinline__ void i4s_copy16(unsigned to, const void* from, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes)
+               : "memory");
 }
 __device__ __forceinline__ void i4s_mma(float* c, const unsigned* a, unsigned b0, unsigned b1) {
   asm volatile(
@@ -39,8 +43,8 @@ template <typename XT> struct I4Frag;
 template <> struct I4Frag<bf16> {
   static constexpr int TERMS = 1;
   uint2 r;
-  __device__ __forceinline__ void load(const bf16* p, bool ok) {
-    r = ok ? *reinterpret_cast<const uint2*>(p) : make_uint2(0, 0);
+  __device__ __forceinline__ void load(const unsigned char* p) {
+    r = *reinterpret_cast<const uint2*>(p);
   }
   __device__ __forceinline__ void terms(unsigned (*b)[2]) const {
     b[0][0] = r.x;
@@ -50,8 +54,8 @@ template <> struct I4Frag<bf16> {
 template <> struct I4Frag<float> {
   static constexpr int TERMS = 3;
   float4 r;
-  __device__ __forceinline__ void load(const float* p, bool ok) {
-    r = ok ? *reinterpret_cast<const float4*>(p) : make_float4(0.f, 0.f, 0.f, 0.f);
+  __device__ __forceinline__ void load(const unsigned char* p) {
+    r = *reinterpret_cast<const float4*>(p);
   }
   __device__ __forceinline__ void terms(unsigned (*b)[2]) const {
     i4_terms2(r.x, r.y, b[0][0], b[1][0], b[2][0]);
@@ -82,92 +86,131 @@ __device__ __forceinline__ void i4s_store(const I4Out& o, size_t r, int j, int N
   else ((bf16*)o.out)[r * N + j] = __float2bfloat16_rn(v);
 }
 
-template <int NT, int GROUP, int S> struct I4SCfg {
+template <typename XT, int NT, int GROUP, int S> struct I4SCfg {
   static constexpr int BYTES = i4_block_words(GROUP) * 4;          // a strip's share of a chunk
-  static constexpr int R = S == 1 ? 8 : 6;                         // stages of a warp's ring
-  static constexpr int RING = I4S_WARPS * R * S * BYTES;
-  static constexpr int SMEM = RING + S * I4S_WARPS * NT * 128 * 4; // and the sums that are joined
+  // a row's activations of a chunk, padded so that the rows of a load meet different banks
+  static constexpr int X_PITCH = I4_CHUNK_K * sizeof(XT) + 16 * sizeof(XT);
+  static constexpr int STAGE = S * BYTES + 8 * NT * X_PITCH;
+  static constexpr int R = NT * sizeof(XT) >= 8 ? 2 : 3;                      // stages of a warp's ring
+  static constexpr int RING = I4S_WARPS * R * STAGE;
+  static constexpr int RED = S * I4S_WARPS * NT * 128 * 4;         // and the sums that are joined
+  static constexpr int SMEM = RING + RED;
+  static_assert(SMEM <= 227 * 1024, "shared memory");
 };
 
 template <typename XT, bool DUAL, int NT, int GROUP, int S>
 __global__ void __launch_bounds__(I4S_THREADS, NT == 1 && sizeof(XT) == 2 ? 2 : 1)
 int4_stream_kernel(const XT* __restrict__ x, const int* __restrict__ rows,
                    const int* __restrict__ offsets, const unsigned* __restrict__ data, I4Out out,
-                   int M_single, int N, int K, int strips, int chunks, int ksplit,
+                   int M_single, int N, int K, int E, int strips, int chunks, int ksplit,
                    int offsets_settled) {
-  typedef I4SCfg<NT, GROUP, S> C;
+  typedef I4SCfg<XT, NT, GROUP, S> C;
   constexpr int NG = 128 / GROUP, PER = GROUP / 16;
   constexpr int TERMS = I4Frag<XT>::TERMS, ACCS = TERMS == 3 ? 2 : 1;
+  // 16-byte pieces of activations: so many lanes take a row's, so many rows go by at once
+  constexpr int PIECES = I4_CHUNK_K * sizeof(XT) / 16, AT_ONCE = 32 / PIECES;
+  constexpr int PASSES = 8 * NT / AT_ONCE;
   static_assert(!DUAL || S == 2, "a gate strip and its up strip");
   extern __shared__ __align__(16) unsigned char smem[];
   float* red = reinterpret_cast<float*>(smem + C::RING);           // [S][warp][NT][4][32]
-  const int e = blockIdx.y;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, t = lane & 3;
   const int tiles = I4S_WARPS / ksplit;
   const int tile = warp / ksplit, ks = warp % ksplit;
   const int pos = blockIdx.x * tiles + tile;
+  // Weights are never written on the device while steps run: the first copies go out before the
+  // wait on the predecessor where the range of rows is known already.
+  const bool early = offsets == nullptr || offsets_settled != 0;
+  if (!early) IX_PDL_WAIT();
+  int e = 0, lo = 0, hi = M_single;
+  if (offsets) {
+    // blockIdx.y counts the groups that have rows (a grid over all of them costs more than their
+    // products where a step's tokens reach few: 4 of 60 experts)
+    int left = blockIdx.y;
+    e = -1;
+    for (int e0 = 0; e0 < E && e < 0; e0 += 32) {
+      const bool some = e0 + lane < E && offsets[e0 + lane + 1] > offsets[e0 + lane];
+      unsigned mask = __ballot_sync(0xffffffffu, some);
+      if (left < __popc(mask)) {
+        for (; left > 0; --left) mask &= mask - 1;
+        e = e0 + __ffs(mask) - 1;
+      } else {
+        left -= __popc(mask);
+      }
+    }
+    if (e < 0) return;
+    lo = offsets[e];
+    hi = offsets[e + 1];
+  }
   // the warp's strips; where there is none its copies come from the first and are not stored
   const size_t pitch = (size_t)strips * C::BYTES;                  // from chunk to chunk
   const unsigned char* base = reinterpret_cast<const unsigned char*>(data) +
-                              (size_t)e * (DUAL ? 2 : 1) * chunks * pitch;
+                              ((size_t)e * (DUAL ? 2 : 1) * chunks + ks) * pitch;
+  const size_t step = pitch * ksplit;
   const unsigned char* from[S];
 #pragma unroll
   for (int s = 0; s < S; ++s) {
     const int strip = DUAL ? pos : S * pos + s;
     from[s] = base + (DUAL && s ? chunks * pitch : 0) +
-              (size_t)(strip < strips ? strip : 0) * C::BYTES;
+              (size_t)(strip < strips ? strip : 0) * C::BYTES + lane * 16;
   }
   // parameters of a strip: 4 NG pieces of 16 bytes, lanes 0.. for the first strip, 16.. for the second
   const bool copies_params = (lane & 15) < 4 * NG && (lane >> 4) < S;
-  const unsigned char* from_params =
-      from[S == 2 ? lane >> 4 : 0] + I4_CODE_WORDS * 4 + (lane & 15) * 16;
-  const unsigned params_at = (S == 2 ? (lane >> 4) * C::BYTES : 0) + I4_CODE_WORDS * 4 + (lane & 15) * 16;
-  unsigned char* ring = smem + warp * (C::R * S * C::BYTES);
-  const unsigned ring_at = (unsigned)__cvta_generic_to_shared(ring);
+  const int params_off = I4_CODE_WORDS * 4 + (lane & 15) * 16 - lane * 16;
+  const unsigned char* from_params = from[S == 2 ? lane >> 4 : 0] + params_off;
+  const unsigned params_at = (S == 2 ? (lane >> 4) * C::BYTES : 0) + params_off;
+  unsigned char* ring = smem + warp * (C::R * C::STAGE);
+  const unsigned ring_at = (unsigned)__cvta_generic_to_shared(ring) + lane * 16;
   const int n = chunks > ks ? (chunks - ks + ksplit - 1) / ksplit : 0;   // chunks of this warp
-  auto fetch = [&](int i) {                        // its i-th chunk, if there is one
-    if (i < n) {
-      const size_t c = (size_t)(ks + i * ksplit) * pitch;
-      const unsigned at = ring_at + (i % C::R) * (S * C::BYTES);
+  // One chunk's codes, or its activations, into stage u (chunks are asked for in order).
+  const unsigned char *next_w[S], *next_params;
+  auto fetch_w = [&](int u) {
+    const unsigned at = ring_at + u * C::STAGE;
 #pragma unroll
-      for (int s = 0; s < S; ++s) {
-        i4s_copy16(at + s * C::BYTES + lane * 16, from[s] + c + lane * 16);
-        i4s_copy16(at + s * C::BYTES + I4_TILE_WORDS * 4 + lane * 16,
-                   from[s] + c + I4_TILE_WORDS * 4 + lane * 16);
-      }
-      if (copies_params) i4s_copy16(at + params_at, from_params + c);
+    for (int s = 0; s < S; ++s) {
+      i4s_copy16(at + s * C::BYTES, next_w[s]);
+      i4s_copy16(at + s * C::BYTES + I4_TILE_WORDS * 4, next_w[s] + I4_TILE_WORDS * 4);
+      next_w[s] += step;
     }
-    asm volatile("cp.async.commit_group;" ::: "memory");
+    if (copies_params) i4s_copy16(at + params_at, next_params);
+    next_params += step;
   };
-  // Weights are never written on the device while steps run: the first copies go out before the
-  // wait on the predecessor where the range of rows is known already.
-  const bool early = offsets == nullptr || offsets_settled != 0;
-  int lo = 0, hi = M_single;
+  auto start_w = [&]() {
+#pragma unroll
+    for (int s = 0; s < S; ++s) next_w[s] = from[s];
+    next_params = from_params;
+  };
   if (early) {
-    if (offsets) {
-      lo = offsets[e];
-      hi = offsets[e + 1];
-    }
-    if (lo >= hi) return;
-    for (int i = 0; i < C::R - 1; ++i) fetch(i);
-  }
-  IX_PDL_WAIT();
-  if (!early) {
-    lo = offsets[e];
-    hi = offsets[e + 1];
-    if (lo >= hi) return;
+    start_w();
+    for (int i = 0; i < C::R - 1; ++i)
+      if (i < n) fetch_w(i);
+    IX_PDL_WAIT();
   }
   for (int r0 = lo; r0 < hi; r0 += 8 * NT) {
-    const XT* xrow[NT];
-    bool xok[NT];
+    // this lane's pieces of the activations: rows r0 + lane / PIECES + AT_ONCE * q.  Rows behind the
+    // last are not copied: what stands there meets columns of the product that are not stored.
+    const int first_k = (lane % PIECES) * (16 / (int)sizeof(XT));
+    const unsigned x_at = ring_at - lane * 16 + S * C::BYTES + (lane / PIECES) * C::X_PITCH +
+                          (lane % PIECES) * 16;
+    const XT* xrow[PASSES];
 #pragma unroll
-    for (int i = 0; i < NT; ++i) {
-      const int r = r0 + i * 8 + g;
-      xok[i] = r < hi;
-      const size_t src = xok[i] ? (rows ? (size_t)rows[r] : (size_t)r) : 0;
-      xrow[i] = x + src * K + t * 4;
+    for (int q = 0; q < PASSES; ++q) {
+      const int r = r0 + lane / PIECES + AT_ONCE * q;
+      const size_t src = r < hi ? (rows ? (size_t)rows[r] : (size_t)r) : 0;
+      xrow[q] = x + src * K + ks * I4_CHUNK_K + first_k;
     }
+    const int here = hi - r0 - lane / PIECES;      // rows left from this lane's first
+    int next_k = ks * I4_CHUNK_K + first_k;
+    auto fetch_x = [&](int u) {
+      const int bytes = next_k < K ? 16 : 0;       // K is a multiple of 8
+#pragma unroll
+      for (int q = 0; q < PASSES; ++q) {
+        if (AT_ONCE * q < here)
+          i4s_copy16(x_at + u * C::STAGE + AT_ONCE * q * C::X_PITCH, xrow[q], bytes);
+        xrow[q] += ksplit * I4_CHUNK_K;
+      }
+      next_k += ksplit * I4_CHUNK_K;
+    };
     float tot[S][NT][4];
 #pragma unroll
     for (int s = 0; s < S; ++s)
@@ -176,34 +219,31 @@ int4_stream_kernel(const XT* __restrict__ x, const int* __restrict__ rows,
 #pragma unroll
         for (int c = 0; c < 4; ++c) tot[s][i][c] = 0.f;
     if (!(early && r0 == lo)) {
-      __syncwarp();                                // the previous pass has read its parameters
-      for (int i = 0; i < C::R - 1; ++i) fetch(i);
+      __syncwarp();                                // the previous pass has read its stages
+      start_w();
+      for (int i = 0; i < C::R - 1; ++i)
+        if (i < n) fetch_w(i);
     }
-    I4Frag<XT> f[8][NT], f_next[8][NT];
-    auto fetch_x = [&](int i) {
-      const int k0 = (ks + i * ksplit) * I4_CHUNK_K;
-#pragma unroll
-      for (int b = 0; b < 8; ++b)
-#pragma unroll
-        for (int j = 0; j < NT; ++j)
-          f_next[b][j].load(xrow[j] + k0 + b * 16, xok[j] && i < n && k0 + b * 16 + t * 4 < K);
-    };
-    fetch_x(0);
+    for (int i = 0; i < C::R - 1; ++i) {
+      if (i < n) fetch_x(i);
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+    int u = 0, ahead = C::R - 1;                   // the stage of chunk i, and of chunk i + R - 1
     for (int i = 0; i < n; ++i) {
       asm volatile("cp.async.wait_group %0;" ::"n"(C::R - 2) : "memory");
-      __syncwarp();            // parameters were copied by other lanes; the last chunk's are read
-      fetch(i + C::R - 1);
-#pragma unroll
-      for (int b = 0; b < 8; ++b)
-#pragma unroll
-        for (int j = 0; j < NT; ++j) f[b][j] = f_next[b][j];
-      fetch_x(i + 1);
-      const unsigned* block = reinterpret_cast<const unsigned*>(ring + (i % C::R) * (S * C::BYTES));
+      __syncwarp();            // pieces were copied by other lanes; the last chunk's stage is read
+      if (i + C::R - 1 < n) {
+        fetch_w(ahead);
+        fetch_x(ahead);
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      const unsigned char* block = ring + u * C::STAGE;
+      const unsigned char* xs = block + S * C::BYTES + g * C::X_PITCH + t * (4 * sizeof(XT));
       uint4 w[S][2];
       unsigned pa[S][NG], pb[S][NG];
 #pragma unroll
       for (int s = 0; s < S; ++s) {
-        const unsigned* at = block + s * (C::BYTES / 4);
+        const unsigned* at = reinterpret_cast<const unsigned*>(block + s * C::BYTES);
         w[s][0] = *reinterpret_cast<const uint4*>(at + lane * 4);
         w[s][1] = *reinterpret_cast<const uint4*>(at + I4_TILE_WORDS + lane * 4);
 #pragma unroll
@@ -225,6 +265,9 @@ int4_stream_kernel(const XT* __restrict__ x, const int* __restrict__ rows,
 #pragma unroll
                 for (int q = 0; q < 4; ++q) acc[a][s][j][q] = 0.f;
         }
+        I4Frag<XT> f[NT];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) f[j].load(xs + j * 8 * C::X_PITCH + b * (16 * sizeof(XT)));
         unsigned a[S][4];
 #pragma unroll
         for (int s = 0; s < S; ++s) {
@@ -239,7 +282,7 @@ int4_stream_kernel(const XT* __restrict__ x, const int* __restrict__ rows,
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
           unsigned xb[TERMS][2];
-          f[b][j].terms(xb);
+          f[j].terms(xb);
 #pragma unroll
           for (int m = TERMS - 1; m >= 0; --m)
 #pragma unroll
@@ -261,6 +304,8 @@ int4_stream_kernel(const XT* __restrict__ x, const int* __restrict__ rows,
           }
         }
       }
+      u = u + 1 == C::R ? 0 : u + 1;
+      ahead = ahead + 1 == C::R ? 0 : ahead + 1;
     }
     // q = 0, 1: column g of the strip, rows 2t and 2t + 1; q = 2, 3: column g + 8
     auto store = [&](int p, int col, int r, float v, float u) {
@@ -312,20 +357,26 @@ struct I4SCall {
 
 template <typename XT, bool DUAL, int NT, int GROUP, int S>
 static int i4s_launch2(const I4SCall& c, cudaStream_t stream) {
-  typedef I4SCfg<NT, GROUP, S> C;
+  typedef I4SCfg<XT, NT, GROUP, S> C;
   const int strips = (int)i4_strips(c.N), chunks = (int)i4_chunks(c.K);
   const int sets = DUAL ? strips : (strips + S - 1) / S;
-  // K is split over the warps of a block until every SM has sixteen warps
+  // K is split over the warps of a block until there are 32 warps for every SM, as long as a warp
+  // keeps four chunks (us at 8 rows, 1 / 2 / 4 / 8 warps: gated 3584 x 20480 42 / 33 / 28 / 30; 25
+  // experts of 2 x 1408 x 2048 34 / 32 / 34 / 42); where that leaves SMs idle it is split further (2048
+  // x 6144 9 / 6.5 / 6.2 / 6.5, 2048 x 2048 8.6 / 5.9 / 4.2 / 3.6).
   int ksplit = 1;
-  while (ksplit < 8 && ksplit < chunks && (long long)sets * c.active * ksplit < 148 * 16) ksplit *= 2;
+  const long long warps = (long long)sets * c.active;
+  while (ksplit < 8 && ksplit < chunks && warps * ksplit < 148 * 32 &&
+         (chunks >= 8 * ksplit || warps * ksplit < 148 * 8))
+    ksplit *= 2;
   const int tiles = I4S_WARPS / ksplit;
   auto kern = int4_stream_kernel<XT, DUAL, NT, GROUP, S>;
   const cudaError_t e =
       cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
   if (e != cudaSuccess) return (int)e;
-  ix_launch(kern, dim3((sets + tiles - 1) / tiles, c.E), dim3(I4S_THREADS), C::SMEM, stream,
+  ix_launch(kern, dim3((sets + tiles - 1) / tiles, c.active), dim3(I4S_THREADS), C::SMEM, stream,
             (const XT*)c.x, c.rows, c.offsets, (const unsigned*)c.data, c.out, c.offsets ? 0 : c.M,
-            c.N, c.K, strips, chunks, ksplit, c.settled);
+            c.N, c.K, c.E, strips, chunks, ksplit, c.settled);
   return ix_launch_status();
 }
 
@@ -341,7 +392,7 @@ static int i4s_launch(const I4SCall& c, cudaStream_t stream) {
 
 // x: [*, K] fp32 or bf16, K a multiple of 8, 16-byte aligned; data as int4_format.cuh lays
 // it out, [E or 2 E matrices]; out: [rows, N] fp32 (wide) or bf16.  offsets == null: one
-// matrix with M rows.  active: how many of the E groups are expected to have rows.
+// matrix with M rows.  active: the most groups that can have rows (0: all).
 // offsets_settled: nonzero when `offsets` was written at least two launches back in the stream.
 IX_API int ix_int4_stream(const void* x, int x_dtype, const int* rows, const int* offsets,
                           const void* data, void* out, int wide, int dual, int M, int N, int K, int E,

@@ -1667,7 +1667,7 @@ def _int4_stream(what, x, rows, offsets, w, num_rows, out_dtype, rows_per_pass, 
     _check(_lib().ix_int4_stream(
         _ptr(x), _dtype_code(x), _ptr(rows), _ptr(offsets), _ptr(w.data),
         _ptr(out), 1 if out_dtype == torch.float32 else 0, w.halves - 1,
-        0 if offsets is not None else num_rows, w.cols, x.shape[1], w.experts, w.group_size,
+        num_rows, w.cols, x.shape[1], w.experts, w.group_size,
         rows_per_pass, active, 1 if offsets_settled else 0, _ptr(row_scale),
         _ACTIVATIONS[activation], _stream()), what)
     _count()
