@@ -102,7 +102,7 @@ template <typename XT, bool DUAL, int NT, int GROUP, int S>
 __global__ void __launch_bounds__(I4S_THREADS, NT == 1 && sizeof(XT) == 2 ? 2 : 1)
 int4_stream_kernel(const XT* __restrict__ x, const int* __restrict__ rows,
                    const int* __restrict__ offsets, const unsigned* __restrict__ data, I4Out out,
-                   int M_single, int N, int K, int E, int strips, int chunks, int ksplit,
+                   int M_single, int N, int K, int E, int strips, int chunks, int klog,
                    int offsets_settled) {
   typedef I4SCfg<XT, NT, GROUP, S> C;
   constexpr int NG = 128 / GROUP, PER = GROUP / 16;
@@ -115,8 +115,8 @@ int4_stream_kernel(const XT* __restrict__ x, const int* __restrict__ rows,
   float* red = reinterpret_cast<float*>(smem + C::RING);           // [S][warp][NT][4][32]
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, t = lane & 3;
-  const int tiles = I4S_WARPS / ksplit;
-  const int tile = warp / ksplit, ks = warp % ksplit;
+  const int ksplit = 1 << klog, tiles = I4S_WARPS >> klog;
+  const int tile = warp >> klog, ks = warp & (ksplit - 1);
   const int pos = blockIdx.x * tiles + tile;
   // Weights are never written on the device while steps run: the first copies go out before the
   // wait on the predecessor where the range of rows is known already.
@@ -146,7 +146,7 @@ int4_stream_kernel(const XT* __restrict__ x, const int* __restrict__ rows,
   const size_t pitch = (size_t)strips * C::BYTES;                  // from chunk to chunk
   const unsigned char* base = reinterpret_cast<const unsigned char*>(data) +
                               ((size_t)e * (DUAL ? 2 : 1) * chunks + ks) * pitch;
-  const size_t step = pitch * ksplit;
+  const size_t step = pitch << klog;
   const unsigned char* from[S];
 #pragma unroll
   for (int s = 0; s < S; ++s) {
@@ -161,7 +161,7 @@ int4_stream_kernel(const XT* __restrict__ x, const int* __restrict__ rows,
   const unsigned params_at = (S == 2 ? (lane >> 4) * C::BYTES : 0) + params_off;
   unsigned char* ring = smem + warp * (C::R * C::STAGE);
   const unsigned ring_at = (unsigned)__cvta_generic_to_shared(ring) + lane * 16;
-  const int n = chunks > ks ? (chunks - ks + ksplit - 1) / ksplit : 0;   // chunks of this warp
+  const int n = (chunks - ks + ksplit - 1) >> klog;   // chunks of this warp
   // One chunk's codes, or its activations, into stage u (chunks are asked for in order).
   const unsigned char *next_w[S], *next_params;
   auto fetch_w = [&](int u) {
@@ -314,7 +314,7 @@ int4_stream_kernel(const XT* __restrict__ x, const int* __restrict__ rows,
       if (j < N) i4s_store<DUAL>(out, r, j, N, v, u);
       if (S == 2 && !DUAL && j + I4_STRIP < N) i4s_store<DUAL>(out, r, j + I4_STRIP, N, u, 0.f);
     };
-    if (ksplit == 1) {
+    if (klog == 0) {
 #pragma unroll
       for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -364,19 +364,19 @@ static int i4s_launch2(const I4SCall& c, cudaStream_t stream) {
   // keeps four chunks (us at 8 rows, 1 / 2 / 4 / 8 warps: gated 3584 x 20480 42 / 33 / 28 / 30; 25
   // experts of 2 x 1408 x 2048 34 / 32 / 34 / 42); where that leaves SMs idle it is split further (2048
   // x 6144 9 / 6.5 / 6.2 / 6.5, 2048 x 2048 8.6 / 5.9 / 4.2 / 3.6).
-  int ksplit = 1;
+  int klog = 0;
   const long long warps = (long long)sets * c.active;
-  while (ksplit < 8 && ksplit < chunks && warps * ksplit < 148 * 32 &&
-         (chunks >= 8 * ksplit || warps * ksplit < 148 * 8))
-    ksplit *= 2;
-  const int tiles = I4S_WARPS / ksplit;
+  while (klog < 3 && (1 << klog) < chunks && (warps << klog) < 148 * 32 &&
+         (chunks >= (8 << klog) || (warps << klog) < 148 * 8))
+    ++klog;
+  const int tiles = I4S_WARPS >> klog;
   auto kern = int4_stream_kernel<XT, DUAL, NT, GROUP, S>;
   const cudaError_t e =
       cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
   if (e != cudaSuccess) return (int)e;
   ix_launch(kern, dim3((sets + tiles - 1) / tiles, c.active), dim3(I4S_THREADS), C::SMEM, stream,
             (const XT*)c.x, c.rows, c.offsets, (const unsigned*)c.data, c.out, c.offsets ? 0 : c.M,
-            c.N, c.K, c.E, strips, chunks, ksplit, c.settled);
+            c.N, c.K, c.E, strips, chunks, klog, c.settled);
   return ix_launch_status();
 }
 
