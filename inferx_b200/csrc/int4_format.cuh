@@ -33,6 +33,27 @@
 // words of a block
 __host__ __device__ constexpr int i4_block_words(int group) { return I4_CODE_WORDS + 16 * (128 / group); }
 
+// A matrix, or one per expert, as the products' entry points take it (filled in by the caller).
+struct I4Weight {
+  const unsigned* data;
+  int N;                               // columns of the product: rows of a matrix
+  int E;                               // experts
+  int group;
+  int dual;                            // a gate and an up matrix per expert
+};
+
+// Shared memory beyond 48 KB has to be asked for once per kernel and device.
+template <typename F> static inline cudaError_t i4_allow_smem(F kern, int bytes, unsigned* done) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const unsigned bit = 1u << (dev & 31);
+  if (*done & bit) return cudaSuccess;
+  const cudaError_t e =
+      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) *done |= bit;
+  return e;
+}
+
 __host__ __device__ static inline long long i4_strips(long long rows) {
   return (rows + I4_STRIP - 1) / I4_STRIP;
 }

@@ -371,8 +371,8 @@ static int i4s_launch2(const I4SCall& c, cudaStream_t stream) {
     ++klog;
   const int tiles = I4S_WARPS >> klog;
   auto kern = int4_stream_kernel<XT, DUAL, NT, GROUP, S>;
-  const cudaError_t e =
-      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+  static unsigned done = 0;
+  const cudaError_t e = i4_allow_smem(kern, C::SMEM, &done);
   if (e != cudaSuccess) return (int)e;
   ix_launch(kern, dim3((sets + tiles - 1) / tiles, c.active), dim3(I4S_THREADS), C::SMEM, stream,
             (const XT*)c.x, c.rows, c.offsets, (const unsigned*)c.data, c.out, c.offsets ? 0 : c.M,
@@ -390,23 +390,23 @@ static int i4s_launch(const I4SCall& c, cudaStream_t stream) {
   return i4s_launch2<XT, DUAL, NT, GROUP, 2>(c, stream);
 }
 
-// x: [*, K] fp32 or bf16, K a multiple of 8, 16-byte aligned; data as int4_format.cuh lays
-// it out, [E or 2 E matrices]; out: [rows, N] fp32 (wide) or bf16.  offsets == null: one
-// matrix with M rows.  active: the most groups that can have rows (0: all).
-// offsets_settled: nonzero when `offsets` was written at least two launches back in the stream.
-IX_API int ix_int4_stream(const void* x, int x_dtype, const int* rows, const int* offsets,
-                          const void* data, void* out, int wide, int dual, int M, int N, int K, int E,
-                          int group, int rows_per_pass, int active, int offsets_settled,
-                          const float* row_scale, int plain,
+// x: [*, K] fp32 or bf16, K a multiple of 8 that ends in the weight's last chunk, 16-byte aligned;
+// out: [rows, N] fp32 (wide) or bf16.  offsets == null: one matrix with M rows.  active: the most
+// groups that can have rows (0: all).  offsets_settled: nonzero when `offsets` was written at least two
+// launches back in the stream.
+IX_API int ix_int4_stream(const I4Weight* w, const void* x, int x_dtype, const int* rows,
+                          const int* offsets, void* out, int wide, int M, int K, int rows_per_pass,
+                          int active, int offsets_settled, const float* row_scale, int plain,
                           cudaStream_t stream) {
+  const int E = w->E, group = w->group, dual = w->dual;
   if ((row_scale && !dual) || (plain && dual)) return IX_ERR_UNSUPPORTED;
-  if (N <= 0 || K <= 0 || E <= 0 || E > 65535) return IX_ERR_SIZE;
+  if (w->N <= 0 || K <= 0 || E <= 0 || E > 65535) return IX_ERR_SIZE;
   if (K % 8 != 0) return IX_ERR_UNSUPPORTED;
   if (!offsets && E != 1) return IX_ERR_SIZE;
   if (!offsets && M <= 0) return IX_OK;
-  if ((uintptr_t)x & 15) return IX_ERR_ALIGN;
+  if (((uintptr_t)x | (uintptr_t)w->data) & 15) return IX_ERR_ALIGN;
   if (active <= 0 || active > E) active = E;
-  const I4SCall c = {x, rows, offsets, data, {out, wide, row_scale, plain}, M, N, K, E, active,
+  const I4SCall c = {x, rows, offsets, w->data, {out, wide, row_scale, plain}, M, w->N, K, E, active,
                      offsets_settled};
   const int nt = rows_per_pass > 16 ? 4 : rows_per_pass > 8 ? 2 : 1;
 #define I4S_GO(T, D, NT, G) return i4s_launch<T, D, NT, G>(c, stream)

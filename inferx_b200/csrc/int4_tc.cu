@@ -704,7 +704,8 @@ static int i4t_launch(const void* x, int Kp, const I4TArgs& p, int sms, cudaStre
   const long long items = tiles * ((p.N + C::F - 1) / C::F) * p.splits;
   if (items > 0x7fffffffLL) return IX_ERR_SIZE;
   auto kern = int4_tc_kernel<TERMS, DUAL, BT, GROUP>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+  static unsigned done = 0;
+  const cudaError_t e = i4_allow_smem(kern, C::SMEM, &done);
   if (e != cudaSuccess) return (int)e;
   const int pairs = sms / 2;
   kern<<<2 * (int)(items < pairs ? items : pairs), I4T_THREADS, C::SMEM, stream>>>(map, p);
@@ -768,24 +769,25 @@ static I4TPlan i4t_plan(int rows, int N, int Kp, int E, bool grouped, bool dual,
 }
 
 // fp32 entries of scratch that a call of these sizes wants (0: none)
-IX_API long long ix_int4_tc_scratch(int rows, int N, int Kp, int E, int grouped, int dual, int terms) {
-  if (rows <= 0 || N <= 0 || Kp <= 0 || E <= 0) return 0;
-  const I4TPlan plan = i4t_plan(rows, N, Kp, E, grouped != 0, dual != 0, terms);
-  return plan.splits > 1 ? (long long)plan.splits * rows * N * (dual ? 2 : 1) : 0;
+IX_API long long ix_int4_tc_scratch(const I4Weight* w, int rows, int Kp, int grouped, int terms) {
+  if (rows <= 0 || w->N <= 0 || Kp <= 0 || w->E <= 0) return 0;
+  const I4TPlan plan = i4t_plan(rows, w->N, Kp, w->E, grouped != 0, w->dual != 0, terms);
+  return plan.splits > 1 ? (long long)plan.splits * rows * w->N * (w->dual ? 2 : 1) : 0;
 }
 
-// x: [rows, Kp] bf16, or [3, rows, Kp] terms of fp32 rows; Kp a multiple of 8 that ends in the last
-// chunk.  out: [rows, N] fp32 (wide) or bf16.  offsets == null: one matrix.  part: scratch of the size
-// that ix_int4_tc_scratch names, or null where it names none.  status: one int, zero before the first
-// call.
-IX_API int ix_int4_tc(const void* x, int terms, const int* offsets, const void* data, void* out,
-                      float* part, int wide, int dual, int rows, int N, int Kp, int E, int group,
-                      const float* row_scale, int plain, int* status, cudaStream_t stream) {
+// x: [rows, Kp] bf16, or [3, rows, Kp] terms of fp32 rows; Kp a multiple of 8 that ends in the weight's
+// last chunk.  out: [rows, N] fp32 (wide) or bf16.  offsets == null: one matrix.  part: scratch of the
+// size that ix_int4_tc_scratch names, or null where it names none.  status: one int, zero before the
+// first call.
+IX_API int ix_int4_tc(const I4Weight* w, const void* x, int terms, const int* offsets, void* out,
+                      float* part, int wide, int rows, int Kp, const float* row_scale, int plain,
+                      int* status, cudaStream_t stream) {
+  const int N = w->N, E = w->E, group = w->group, dual = w->dual;
   if ((row_scale && !dual) || (plain && dual)) return IX_ERR_UNSUPPORTED;
   if (rows <= 0) return IX_OK;
   if (N <= 0 || Kp <= 0 || E <= 0 || status == nullptr) return IX_ERR_SIZE;
   if (Kp % 8 != 0 || E > I4T_MAX_EXPERTS || (!offsets && E != 1)) return IX_ERR_UNSUPPORTED;
-  if (((uintptr_t)x | (uintptr_t)data) & 15) return IX_ERR_ALIGN;
+  if (((uintptr_t)x | (uintptr_t)w->data) & 15) return IX_ERR_ALIGN;
   if (3LL * rows > 0x7fffffffLL || N > 0x3fffff00) return IX_ERR_SIZE;
   const I4TPlan plan = i4t_plan(rows, N, Kp, E, offsets != nullptr, dual != 0, terms);
   if (plan.splits > 1) {
@@ -794,7 +796,7 @@ IX_API int ix_int4_tc(const void* x, int terms, const int* offsets, const void* 
     part = nullptr;
   }
   const int chunks = (int)i4_chunks(Kp);
-  const I4TArgs p = {offsets, (const unsigned*)data, out, part, wide, row_scale, plain, rows, N,
+  const I4TArgs p = {offsets, w->data, out, part, wide, row_scale, plain, rows, N,
                      (int)i4_strips(N), chunks, E, plan.tile_rows, plan.splits,
                      (chunks + plan.splits - 1) / plan.splits, rows, status};
   const int sms = i4t_sms();

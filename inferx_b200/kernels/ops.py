@@ -1510,6 +1510,12 @@ INT4_GROUPS = (32, 64, 128)
 INT4_LAYOUT_ROWS, INT4_LAYOUT_K = 16, 128     # a strip of rows, a chunk of k
 
 
+class _Int4Record(ctypes.Structure):
+    """What the products' entry points want to know of a weight (csrc/int4_format.cuh)."""
+    _fields_ = [("data", ctypes.c_void_p), ("cols", ctypes.c_int), ("experts", ctypes.c_int),
+                ("group", ctypes.c_int), ("dual", ctypes.c_int)]
+
+
 class Int4Weight:
     """A matrix ``[rows, K]``, or one per expert ``[E, rows, K]``, in four bits: per row and
     group of ``group_size`` entries along K a bfloat16 scale and a zero point in 0..15, per entry
@@ -1517,26 +1523,24 @@ class Int4Weight:
     ``pack_int4``; ``linear`` and the gated and grouped products take it where they take a
     matrix.  ``halves`` is 2 where the rows are a gate matrix and then an up matrix of the same
     size, which the gated products want, and 1 otherwise.  ``data`` is an int32 tensor in the
-    kernels' own layout."""
+    kernels' own layout; ``cols`` counts a product's output columns, the rows of one half."""
 
-    __slots__ = ("shape", "halves", "group_size", "data")
+    __slots__ = ("shape", "halves", "group_size", "data", "experts", "cols", "inner", "per_expert",
+                 "device_index", "_record", "_at")
 
     def __init__(self, shape, halves: int, group_size: int, data: torch.Tensor):
         self.shape = torch.Size(shape)
         self.halves, self.group_size, self.data = halves, group_size, data
+        self.experts = self.shape[0] if len(self.shape) == 3 else 1
+        self.per_expert = len(self.shape) == 3
+        self.cols, self.inner = self.shape[-2] // halves, self.shape[-1]
+        self.device_index = data.get_device()
+        self._record = _Int4Record(data.data_ptr(), self.cols, self.experts, group_size, halves - 1)
+        self._at = ctypes.addressof(self._record)
 
     @property
     def device(self):
         return self.data.device
-
-    @property
-    def experts(self) -> int:
-        return self.shape[0] if len(self.shape) == 3 else 1
-
-    @property
-    def cols(self) -> int:
-        """Output columns of a product: the rows of one half."""
-        return self.shape[-2] // self.halves
 
     @property
     def nbytes(self) -> int:
@@ -1568,9 +1572,9 @@ def _int4_empty(what: str, shape, group_size: int, halves: int, device) -> Int4W
 
 def _on_current_device(what: str, *tensors):
     """Kernels launch on the current device's stream: operands of another one are refused."""
-    now = torch.cuda.current_device()
+    now = _raw_device() if _raw_device is not None else torch.cuda.current_device()
     for t in tensors:
-        if t is not None and t.device.index != now:
+        if t is not None and t.get_device() != now:
             raise KernelError(f"{what}: an operand is on {t.device}, the current device is "
                               f"cuda:{now}")
 
@@ -1630,18 +1634,43 @@ def unpack_int4(w: Int4Weight):
     return codes, scales, zeros
 
 
-def _int4_operands(what: str, x: torch.Tensor, w: Int4Weight, halves: int, dims: int,
-                   *others) -> int:
-    """The checks that every product with an ``Int4Weight`` makes; the code of x's type."""
+_INT4_ENTRIES = {}
+
+
+def _int4_entry(name: str):
+    """A product's entry point, its argument types declared once (a call then passes plain
+    integers: a few microseconds less than wrapping each)."""
+    fn = _INT4_ENTRIES.get(name)
+    if fn is None:
+        p, i = ctypes.c_void_p, ctypes.c_int
+        fn = getattr(_lib(), name)
+        fn.argtypes = {"ix_int4_stream": [p, p, i, p, p, p, i, i, i, i, i, i, p, i, p],
+                       "ix_int4_tc": [p, p, i, p, p, p, i, i, i, p, i, p, p],
+                       "ix_int4_tc_scratch": [p, i, i, i, i]}[name]
+        if name == "ix_int4_tc_scratch":
+            fn.restype = ctypes.c_longlong
+        _INT4_ENTRIES[name] = fn
+    return fn
+
+
+def _at(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+def _int4_operands(what: str, x: torch.Tensor, w: Int4Weight, halves: int, per_expert: bool,
+                   *others) -> None:
+    """The checks that every product with an ``Int4Weight`` makes."""
     _chk("x", x)
-    code = _dtype_code(x)
-    _on_current_device(what, x, w.data, *others)
-    if x.dim() != 2 or len(w.shape) != dims or x.shape[1] != w.shape[-1]:
+    _dtype_code(x)
+    now = _raw_device() if _raw_device is not None else torch.cuda.current_device()
+    if x.get_device() != now or w.device_index != now:
+        _on_current_device(what, x, w.data)
+    _on_current_device(what, *others)
+    if x.dim() != 2 or w.per_expert != per_expert or x.shape[1] != w.inner:
         raise KernelError(f"{what}: activations {list(x.shape)} against weights "
                           f"{list(w.shape)}")
     if w.halves != halves:
         raise KernelError(f"{what}: weights of {w.halves} halves, {halves} wanted")
-    return code
 
 
 def _int4_rows(x: torch.Tensor, rows: Optional[torch.Tensor], terms: int) -> torch.Tensor:
@@ -1660,62 +1689,68 @@ def _int4_rows(x: torch.Tensor, rows: Optional[torch.Tensor], terms: int) -> tor
 def _int4_stream(what, x, rows, offsets, w, num_rows, out_dtype, rows_per_pass, active=0,
                  offsets_settled=False, row_scale=None, activation=None):
     """Few rows: the codes stream past the activations (csrc/int4_stream.cu)."""
-    if x.shape[1] % 8 or x.data_ptr() % 16:
+    at = x.data_ptr()
+    if w.inner % 8 or at % 16:
         x, rows = _int4_rows(x, rows, 1), None
-        offsets_settled = False            # one launch more in front of this one
-    out = torch.empty((num_rows, w.cols), dtype=out_dtype, device=x.device)
-    _check(_lib().ix_int4_stream(
-        _ptr(x), _dtype_code(x), _ptr(rows), _ptr(offsets), _ptr(w.data),
-        _ptr(out), 1 if out_dtype == torch.float32 else 0, w.halves - 1,
-        num_rows, w.cols, x.shape[1], w.experts, w.group_size,
-        rows_per_pass, active, 1 if offsets_settled else 0, _ptr(row_scale),
-        _ACTIVATIONS[activation], _stream()), what)
+        at = x.data_ptr()
+    out = x.new_empty((num_rows, w.cols), dtype=out_dtype)
+    _check(_int4_entry("ix_int4_stream")(
+        w._at, at, _dtype_code(x), _at(rows), _at(offsets), out.data_ptr(),
+        1 if out_dtype is torch.float32 else 0, num_rows, x.shape[1], rows_per_pass, active,
+        1 if offsets_settled else 0, _at(row_scale), _ACTIVATIONS[activation], _stream()), what)
     _count()
     return out
 
 
-# Up to this many rows of one matrix, or rows an expert on average, the codes stream past them;
-# beyond, the tcgen05 kernel.
-INT4_STREAM_ROWS = 32
-INT4_STREAM_ROWS_PER_GROUP = 2
-INT4_TC_MAX_EXPERTS = 1024
+INT4_MAX_EXPERTS = 1024      # the tensor-core kernel's prefix of tiles lives in shared memory
 
 
 def _int4_tc(what, x, rows, offsets, w, num_rows, out_dtype, row_scale=None, activation=None):
     """Many rows, on the 5th-generation tensor cores (csrc/int4_tc.cu)."""
     terms = 3 if x.dtype == torch.float32 else 1
-    if terms == 3 or x.shape[1] % 8 or x.data_ptr() % 16:
+    if terms == 3 or w.inner % 8 or x.data_ptr() % 16:
         x = _int4_rows(x, rows, terms)
     elif rows is not None:
         x = gather_rows(x, rows)
     out = torch.empty((num_rows, w.cols), dtype=out_dtype, device=x.device)
-    lib = _lib()
-    lib.ix_int4_tc_scratch.restype = ctypes.c_longlong
-    need = lib.ix_int4_tc_scratch(num_rows, w.cols, x.shape[-1], w.experts,
-                                  0 if offsets is None else 1, w.halves - 1, terms)
+    need = _int4_entry("ix_int4_tc_scratch")(w._at, num_rows, x.shape[-1],
+                                             0 if offsets is None else 1, terms)
     part = torch.empty(need, dtype=torch.float32, device=x.device) if need else None
-    _check(lib.ix_int4_tc(
-        _ptr(x), terms, _ptr(offsets), _ptr(w.data), _ptr(out), _ptr(part),
-        1 if out_dtype == torch.float32 else 0, w.halves - 1, num_rows, w.cols, x.shape[-1],
-        w.experts, w.group_size, _ptr(row_scale), _ACTIVATIONS[activation],
-        _ptr(_tc_status(x.device)), _stream()), what)
+    _check(_int4_entry("ix_int4_tc")(
+        w._at, x.data_ptr(), terms, _at(offsets), out.data_ptr(), _at(part),
+        1 if out_dtype is torch.float32 else 0, num_rows, x.shape[-1], _at(row_scale),
+        _ACTIVATIONS[activation], _tc_status(x.device).data_ptr(), _stream()), what)
     _count()
     return out
+
+
+# One matrix: the streaming kernel reads the codes once for every 32 rows (16 in 32 bits) and its
+# time goes by rows x bytes; the tensor-core kernel has some 10 to 16 us to begin and end with.
+# us, streaming / tensor cores: 2048 x 2048 64 rows 8.6 / 11.4, 128 rows 15.0 / 15.7, 192 rows 21.8 /
+# 15.9; 2048 x 6144 32 rows 13.1 / 15.8, 48 rows 22.1 / 15.9; gated 2048 x 5632 16 rows 12.1 / 16.1,
+# 32 rows 17.0 / 16.4; 32-bit 2048 x 2048 32 rows 10.7 / 14.3, 64 rows 19.4 / 16.1.
+INT4_STREAM_ROWS = 16
+INT4_STREAM_ROW_BYTES = {torch.bfloat16: 250e6, torch.float32: 110e6}
+# Experts (60 of 2 x 1408 x 2048 and back, us, streaming 8 / 16 rows a pass / tensor cores): 6.4 rows
+# an expert 115 / 128 / 172, 8.5 rows 136 / 129 / 172, 12.8 rows 176 / 144 / 172; 32-bit 6.4 rows
+# 210 / 262 / 251, 8.5 rows 272 / 265 / 252.
+INT4_STREAM_ROWS_PER_EXPERT = {torch.bfloat16: 12.0, torch.float32: 7.0}
+INT4_PASS8_ROWS_PER_EXPERT = 7.0
 
 
 def _int4_product(what: str, x: torch.Tensor, w: Int4Weight, halves: int,
                   out_dtype: Optional[torch.dtype] = None, activation: Optional[str] = None):
     """One matrix: x . w^T, gated where there are two halves."""
-    _int4_operands(what, x, w, halves, 2)
+    _int4_operands(what, x, w, halves, False)
     out_dtype = out_dtype or x.dtype
     if out_dtype not in (torch.float32, x.dtype):
         raise KernelError(f"{what}: results in {out_dtype} from activations in {x.dtype}")
     M = x.shape[0]
-    if M == 0:
-        return torch.empty((0, w.cols), dtype=out_dtype, device=x.device)
-    if M > INT4_STREAM_ROWS:
-        return _int4_tc(what, x, None, None, w, M, out_dtype, activation=activation)
-    return _int4_stream(what, x, None, None, w, M, out_dtype, M, activation=activation)
+    if M <= INT4_STREAM_ROWS or M * w.data.nbytes <= INT4_STREAM_ROW_BYTES[x.dtype]:
+        if M == 0:
+            return torch.empty((0, w.cols), dtype=out_dtype, device=x.device)
+        return _int4_stream(what, x, None, None, w, M, out_dtype, M, activation=activation)
+    return _int4_tc(what, x, None, None, w, M, out_dtype, activation=activation)
 
 
 def _int4_grouped(what: str, x: torch.Tensor, rows: Optional[torch.Tensor],
@@ -1725,17 +1760,18 @@ def _int4_grouped(what: str, x: torch.Tensor, rows: Optional[torch.Tensor],
     """One matrix per expert, ragged rows."""
     _chk("rows", rows, torch.int32, optional=True)
     _chk("offsets", offsets, torch.int32)
-    _int4_operands(what, x, w, halves, 3, rows, offsets, row_scale)
+    _int4_operands(what, x, w, halves, True, rows, offsets, row_scale)
     A = x.shape[0] if rows is None else rows.numel()
     if offsets.numel() != w.experts + 1:
         raise KernelError(f"{what}: offsets must have one entry per expert plus one")
     if A == 0:
         return torch.empty((0, w.cols), dtype=x.dtype, device=x.device)
     per = A / w.experts
-    if per > INT4_STREAM_ROWS_PER_GROUP and w.experts <= INT4_TC_MAX_EXPERTS:
+    if per > INT4_STREAM_ROWS_PER_EXPERT[x.dtype] and w.experts <= INT4_MAX_EXPERTS:
         return _int4_tc(what, x, rows, offsets, w, A, x.dtype, row_scale=row_scale,
                         activation=activation)
-    return _int4_stream(what, x, rows, offsets, w, A, x.dtype, 8 if per <= 2 else 16,
+    return _int4_stream(what, x, rows, offsets, w, A, x.dtype,
+                        8 if per <= INT4_PASS8_ROWS_PER_EXPERT else 16,
                         active=min(w.experts, A), offsets_settled=offsets_settled,
                         row_scale=row_scale, activation=activation)
 
