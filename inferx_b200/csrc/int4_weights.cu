@@ -12,23 +12,34 @@
 
 #define I4_WARPS 8
 
-// The nearest whole number to v / s (ties to even) for |v| <= 16 s.  v of 24 bits and s of 8: the
-// quotient can round onto a half, the remainder cannot.
-__device__ __forceinline__ float i4_rint_ratio(float v, float s) {
-  float q = rintf(__fdiv_rn(v, s));
-  const float left = fmaf(-q, s, v), half = 0.5f * s;
-  if (left > half) q += 1.f;
-  if (left < -half) q -= 1.f;
+// The nearest whole number to v / s (ties to even) for |v| <= 16 s, r near 1 / s.  The product is off by
+// a step at most, and the remainder (exact: v has 24 bits, s has 8) says which way.
+__device__ __forceinline__ int i4_rint_ratio(float v, float s, float r) {
+  const float t = fmaf(v, r, 12582912.f);          // its last bit is 1: a whole number in the low bits
+  int q = __float_as_int(t) - 0x4b400000;
+  const float left = fmaf(12582912.f - t, s, v), half = 0.5f * s;
+  if (fabsf(left) >= half) {
+    const bool odd = q & 1;
+    if (left > half || (left == half && odd)) ++q;
+    else if (left < -half || (left == -half && odd)) --q;
+  }
   return q;
 }
 
-// (hi - lo) / 15 in 64 bits, cut to 32 with the last bit set where something was cut off, then
-// rounded to bfloat16: one rounding in all.
+// (hi - lo) / 15 rounded once to bfloat16.  In 32 bits the quotient is off by less than two of its
+// steps, which matters only where it lies as near to the middle of two bfloat16 numbers (or is too small
+// for 24 bits): there it is formed in 64 bits, cut to 32 with the last bit set where something was cut
+// off, and rounded from that.
 __device__ __forceinline__ bf16 i4_group_scale(float lo, float hi) {
-  const double q = ((double)hi - (double)lo) / 15.0;
-  unsigned u = __float_as_uint(__double2float_rz(q));
-  if ((double)__uint_as_float(u) != q) u |= 1u;
-  return __float2bfloat16_rn(__uint_as_float(u));
+  float t = __fdiv_rn(hi - lo, 15.f);
+  const int from_middle = (int)(__float_as_uint(t) & 0xffffu) - 0x8000;
+  if ((unsigned)(from_middle + 4) <= 8u || t < 1e-30f || t > 1e37f) {
+    const double q = ((double)hi - (double)lo) / 15.0;
+    unsigned u = __float_as_uint(__double2float_rz(q));
+    if ((double)__uint_as_float(u) != q) u |= 1u;
+    t = __uint_as_float(u);
+  }
+  return __float2bfloat16_rn(t);
 }
 
 __device__ __forceinline__ unsigned i4_param(bf16 scale, int zero) {
@@ -54,34 +65,55 @@ __device__ __forceinline__ size_t i4_block(const I4Place& p, int strips, int chu
 }
 
 // The 32 entries of a row that a lane of `t` holds of a chunk, four of every sixteen, from `src` (the
-// row, or null: zeros).
-template <typename T>
-__device__ __forceinline__ void i4_row_entries(const T* src, int k0, int K, int t, bool vec,
-                                               float* v) {
+// row, or null: zeros), in their own type: 16 registers of bfloat16 pairs leave room for twice the warps
+// that 32 numbers would.
+template <typename T> struct I4Entries;
+template <> struct I4Entries<float> {
+  float v[32];
+  __device__ __forceinline__ float at(int i) const { return v[i]; }
+  __device__ __forceinline__ void load(const float* src, int k0, int K, int t, bool vec) {
 #pragma unroll
-  for (int b = 0; b < 8; ++b) {                    // blocks of 16 k
-    const int k = k0 + b * 16 + t * 4;
-    if (vec && src && k < K) {                     // K is a multiple of 4
-      if (sizeof(T) == 2) {
-        const uint2 r = *reinterpret_cast<const uint2*>(src + k);
-        v[b * 4] = __uint_as_float(r.x << 16);
-        v[b * 4 + 1] = __uint_as_float(r.x & 0xffff0000u);
-        v[b * 4 + 2] = __uint_as_float(r.y << 16);
-        v[b * 4 + 3] = __uint_as_float(r.y & 0xffff0000u);
-      } else {
-        const float4 r = *reinterpret_cast<const float4*>(src + k);
+    for (int b = 0; b < 8; ++b) {                  // blocks of 16 k
+      const int k = k0 + b * 16 + t * 4;
+      if (vec) {                                   // K is a multiple of 4
+        const float4 r = src && k < K ? *reinterpret_cast<const float4*>(src + k)
+                                      : make_float4(0.f, 0.f, 0.f, 0.f);
         v[b * 4] = r.x;
         v[b * 4 + 1] = r.y;
         v[b * 4 + 2] = r.z;
         v[b * 4 + 3] = r.w;
-      }
-    } else {
+      } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        v[b * 4 + i] = (src && k + i < K) ? to_f32<T>(src[k + i]) : 0.f;
+        for (int i = 0; i < 4; ++i) v[b * 4 + i] = src && k + i < K ? src[k + i] : 0.f;
+      }
     }
   }
-}
+};
+template <> struct I4Entries<bf16> {
+  unsigned v[16];
+  __device__ __forceinline__ float at(int i) const {
+    return __uint_as_float((i & 1) ? v[i >> 1] & 0xffff0000u : v[i >> 1] << 16);
+  }
+  __device__ __forceinline__ void load(const bf16* src, int k0, int K, int t, bool vec) {
+    const unsigned short* bits = reinterpret_cast<const unsigned short*>(src);
+#pragma unroll
+    for (int b = 0; b < 8; ++b) {
+      const int k = k0 + b * 16 + t * 4;
+      if (vec) {
+        const uint2 r = src && k < K ? *reinterpret_cast<const uint2*>(bits + k) : make_uint2(0, 0);
+        v[b * 2] = r.x;
+        v[b * 2 + 1] = r.y;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const unsigned lo = src && k + 2 * i < K ? bits[k + 2 * i] : 0u;
+          const unsigned hi = src && k + 2 * i + 1 < K ? bits[k + 2 * i + 1] : 0u;
+          v[b * 2 + i] = lo | (hi << 16);
+        }
+      }
+    }
+  }
+};
 
 // codes of rows g and g + 8 (32 each, in the order of i4_row_entries) to the lane's words
 __device__ __forceinline__ void i4_store_words(unsigned* dst, int lane, const unsigned char* ca,
@@ -103,7 +135,7 @@ __device__ __forceinline__ void i4_store_words(unsigned* dst, int lane, const un
 }
 
 template <typename T, int GROUP>
-__global__ void __launch_bounds__(I4_WARPS * 32)
+__global__ void __launch_bounds__(I4_WARPS * 32, sizeof(T) == 2 ? 4 : 2)
 i4_quantize_kernel(const T* __restrict__ w, unsigned* __restrict__ data,
                    long long matrices, int rows, int K, int strips,
                    int chunks, int vec) {
@@ -113,45 +145,65 @@ i4_quantize_kernel(const T* __restrict__ w, unsigned* __restrict__ data,
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int k0 = p.chunk * I4_CHUNK_K;
   const size_t block = i4_block(p, strips, chunks) * i4_block_words(GROUP);
-  unsigned char code[2][32];
+  I4Entries<T> v[2];
 #pragma unroll
   for (int side = 0; side < 2; ++side) {
     const int row = p.strip * I4_STRIP + g + side * 8;
-    const T* src = row < rows ? w + ((size_t)p.m * rows + row) * K : nullptr;
-    float v[32];
-    i4_row_entries<T>(src, k0, K, t, vec != 0, v);
+    v[side].load(row < rows ? w + ((size_t)p.m * rows + row) * K : nullptr, k0, K, t, vec != 0);
+  }
+  unsigned word[8];                                // of sixteen k each
+#pragma unroll
+  for (int side = 0; side < 2; ++side) {
 #pragma unroll
     for (int n = 0; n < NG; ++n) {
-      float lo = 0.f, hi = 0.f;
-      bool bad = false;
+      const int first = n * PER * 8;
+      float lo = 0.f, hi = 0.f, odd_one = 0.f;     // the last is NaN where an entry is not finite
 #pragma unroll
       for (int i = 0; i < PER * 8; ++i) {
-        const float e = v[n * PER * 8 + i];
+        const float e = v[side].at(first + i);
         lo = fminf(lo, e);
         hi = fmaxf(hi, e);
-        bad |= !(fabsf(e) < INFINITY);
+        odd_one = fmaf(e, 0.f, odd_one);
       }
 #pragma unroll
       for (int o = 1; o < 4; o <<= 1) {
         lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
         hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-        bad |= __shfl_xor_sync(0xffffffffu, (int)bad, o) != 0;
+        odd_one += __shfl_xor_sync(0xffffffffu, odd_one, o);
       }
-      bf16 scale = bad ? __ushort_as_bfloat16(0x7fc0) : i4_group_scale(lo, hi);
-      const float s = __bfloat162float(scale);
+      const bf16 scale = odd_one != 0.f ? __ushort_as_bfloat16(0x7fc0) : i4_group_scale(lo, hi);
+      float s = __bfloat162float(scale);
       const bool some = s > 0.f;                   // false for 0 and for NaN
-      const float zero = some ? fminf(fmaxf(i4_rint_ratio(-lo, s), 0.f), 15.f) : 0.f;
+      int zero = 0;
+      // (so that 1 / s is a number, a group whose scale is tiny is taken 2^100 times as large)
+      auto quantize = [&](float up) {
+        s *= up;
+        const float r = some ? __frcp_rn(s) : 0.f;
+        zero = some ? min(max(i4_rint_ratio(-lo * up, s, r), 0), 15) : 0;
 #pragma unroll
-      for (int i = 0; i < PER * 8; ++i) {
-        const int at = n * PER * 8 + i;
-        const float c = fminf(fmaxf(i4_rint_ratio(v[at], s) + zero, 0.f), 15.f);
-        code[side][at] = some ? (unsigned char)(int)c : 0;
-      }
+        for (int i = 0; i < PER * 2; ++i) {
+          unsigned c[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float e = v[side].at(first + 4 * i + j) * up;
+            const int q = min(max(i4_rint_ratio(e, s, r) + zero, 0), 15);
+            c[j] = some ? (unsigned)q : 0u;
+          }
+          const unsigned half = (c[0] | (c[1] << 16)) | ((c[2] << 8) | (c[3] << 24));
+          unsigned& at = word[n * PER * 2 + i];
+          at = side ? at | (half << 4) : half;
+        }
+      };
+      if (s < 1e-30f) quantize(1.2676506e30f);
+      else quantize(1.f);
       if (t == 0)
-        data[block + I4_CODE_WORDS + (g + side * 8) * NG + n] = i4_param(scale, (int)zero);
+        data[block + I4_CODE_WORDS + (g + side * 8) * NG + n] = i4_param(scale, zero);
     }
   }
-  i4_store_words(data + block, lane, code[0], code[1]);
+#pragma unroll
+  for (int tile = 0; tile < 2; ++tile)
+    *reinterpret_cast<uint4*>(data + block + tile * I4_TILE_WORDS + lane * 4) = make_uint4(
+        word[tile * 4], word[tile * 4 + 1], word[tile * 4 + 2], word[tile * 4 + 3]);
 }
 
 // Codes, scales and zero points of a caller's own into the layout.
@@ -203,7 +255,7 @@ template <int GROUP>
 __global__ void __launch_bounds__(I4_WARPS * 32)
 i4_unpack_kernel(const unsigned* __restrict__ data, unsigned char* __restrict__ out, bf16* __restrict__ scales,
                  unsigned char* __restrict__ zeros, long long matrices, int rows, int K, int strips,
-                 int chunks, int vec) {
+                 int chunks, int whole) {
   constexpr int NG = 128 / GROUP;
   I4Place p;
   if (!i4_place(p, matrices, strips, chunks)) return;
@@ -218,25 +270,45 @@ i4_unpack_kernel(const unsigned* __restrict__ data, unsigned char* __restrict__ 
 #pragma unroll
   for (int side = 0; side < 2; ++side) {
     const int row = p.strip * I4_STRIP + g + side * 8;
-    if (row >= rows) continue;
     const size_t r = (size_t)p.m * rows + row;
 #pragma unroll
-    for (int b = 0; b < 8; ++b) {
-      const int k = k0 + b * 16 + t * 4;
-      const uint4 q = w[b >> 2];
-      const unsigned u = ((b & 3) == 0 ? q.x : (b & 3) == 1 ? q.y : (b & 3) == 2 ? q.z : q.w) >>
-                         (4 * side);
-      // four codes of the row out of a word
-      const unsigned o = (u & 15) | ((u >> 16 & 15) << 8) | ((u >> 8 & 15) << 16) |
-                         ((u >> 24 & 15) << 24);
-      if (vec && k < K) {
-        *reinterpret_cast<unsigned*>(out + r * K + k) = o;
-      } else {
+    for (int h = 0; h < 2; ++h) {                  // 64 k: a lane's four codes of each sixteen
+      const unsigned from[4] = {w[h].x, w[h].y, w[h].z, w[h].w};
+      unsigned o[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (k + i < K) out[r * K + k + i] = (unsigned char)(o >> (8 * i));
+      for (int j = 0; j < 4; ++j) {
+        const unsigned u = from[j] >> (4 * side);
+        o[j] = __byte_perm(u & 0x0f0f0f0fu, 0, 0x3120);
+      }
+      if (whole) {
+        // the four lanes of a row trade, so that lane t has sixteen codes beside each other
+        const bool up = t & 2, right = t & 1;
+        unsigned a0 = up ? o[0] : o[2], a1 = up ? o[1] : o[3];
+        a0 = __shfl_xor_sync(0xffffffffu, a0, 2);
+        a1 = __shfl_xor_sync(0xffffffffu, a1, 2);
+        const unsigned m[4] = {up ? a0 : o[0], up ? a1 : o[1], up ? o[2] : a0, up ? o[3] : a1};
+        unsigned b0 = right ? m[0] : m[1], b1 = right ? m[2] : m[3];
+        b0 = __shfl_xor_sync(0xffffffffu, b0, 1);
+        b1 = __shfl_xor_sync(0xffffffffu, b1, 1);
+        const uint4 r4 = make_uint4(right ? b0 : m[0], right ? m[1] : b0, right ? b1 : m[2],
+                                    right ? m[3] : b1);
+        const int k = k0 + h * 64 + t * 16;
+        if (row < rows && k < K) *reinterpret_cast<uint4*>(out + r * K + k) = r4;
+      } else if (row < rows) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int k = k0 + h * 64 + j * 16 + t * 4;
+          if (K % 4 == 0 && ((uintptr_t)out & 3) == 0) {
+            if (k < K) *reinterpret_cast<unsigned*>(out + r * K + k) = o[j];
+            continue;
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (k + i < K) out[r * K + k + i] = (unsigned char)(o[j] >> (8 * i));
+        }
       }
     }
+    if (row >= rows) continue;
     for (int n = t; n < NG; n += 4) {
       const int group = p.chunk * NG + n;
       if (group >= groups) continue;
@@ -303,10 +375,10 @@ IX_API int ix_int4_unpack(const void* data, void* out, void* scales,
   unsigned grid;
   const int rc = i4_grid(matrices, rows, K, strips, chunks, grid);
   if (rc != IX_OK) return rc;
-  const int vec = K % 4 == 0 && ((uintptr_t)out & 3) == 0;
+  const int whole = K % 16 == 0 && ((uintptr_t)out & 15) == 0;
   I4_GROUPS(G, i4_unpack_kernel<G><<<grid, I4_WARPS * 32, 0, stream>>>(
                    (const unsigned*)data, (unsigned char*)out, (bf16*)scales,
-                   (unsigned char*)zeros, matrices, rows, K, strips, chunks, vec));
+                   (unsigned char*)zeros, matrices, rows, K, strips, chunks, whole));
   return ix_launch_status();
 }
 

@@ -1535,8 +1535,16 @@ class Int4Weight:
         self.per_expert = len(self.shape) == 3
         self.cols, self.inner = self.shape[-2] // halves, self.shape[-1]
         self.device_index = data.get_device()
-        self._record = _Int4Record(data.data_ptr(), self.cols, self.experts, group_size, halves - 1)
-        self._at = ctypes.addressof(self._record)
+        self._record = None
+
+    @property
+    def at(self) -> int:
+        """Where the record is that a product's entry point reads."""
+        if self._record is None:
+            self._record = _Int4Record(self.data.data_ptr(), self.cols, self.experts,
+                                       self.group_size, self.halves - 1)
+            self._at = ctypes.addressof(self._record)
+        return self._at
 
     @property
     def device(self):
@@ -1588,9 +1596,9 @@ def quantize_int4(w: torch.Tensor, group_size: int = 128, halves: int = 1) -> In
     code = _dtype_code(w)
     _on_current_device("quantize_int4", w)
     q = _int4_empty("quantize_int4", w.shape, group_size, halves, w.device)
-    _check(_lib().ix_int4_quantize(_ptr(w), code, _ptr(q.data),
-                                   ctypes.c_longlong(q.experts * halves), q.cols, w.shape[-1],
-                                   group_size, _stream()), "quantize_int4")
+    _check(_int4_entry("ix_int4_quantize")(w.data_ptr(), code, q.data.data_ptr(),
+                                           q.experts * halves, q.cols, q.inner, group_size,
+                                           _stream()), "quantize_int4")
     _count()
     return q
 
@@ -1611,9 +1619,9 @@ def pack_int4(codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor,
                           f"{list(scales.shape)} and {list(zeros.shape)}")
     if int(torch.maximum(codes.max(), zeros.max())) > 15:
         raise KernelError("pack_int4: codes and zeros must lie in 0..15")
-    _check(_lib().ix_int4_pack(_ptr(codes), _ptr(scales), _ptr(zeros), _ptr(q.data),
-                               ctypes.c_longlong(q.experts * halves), q.cols,
-                               codes.shape[-1], group_size, _stream()), "pack_int4")
+    _check(_int4_entry("ix_int4_pack")(codes.data_ptr(), scales.data_ptr(), zeros.data_ptr(),
+                                       q.data.data_ptr(), q.experts * halves, q.cols, q.inner,
+                                       group_size, _stream()), "pack_int4")
     _count()
     return q
 
@@ -1627,9 +1635,9 @@ def unpack_int4(w: Int4Weight):
     codes = torch.empty(w.shape, dtype=torch.uint8, device=w.device)
     scales = torch.empty(groups, dtype=torch.bfloat16, device=w.device)
     zeros = torch.empty(groups, dtype=torch.uint8, device=w.device)
-    _check(_lib().ix_int4_unpack(_ptr(w.data), _ptr(codes), _ptr(scales),
-                                 _ptr(zeros), ctypes.c_longlong(w.experts * w.halves), w.cols,
-                                 w.shape[-1], w.group_size, _stream()), "unpack_int4")
+    _check(_int4_entry("ix_int4_unpack")(w.data.data_ptr(), codes.data_ptr(), scales.data_ptr(),
+                                         zeros.data_ptr(), w.experts * w.halves, w.cols, w.inner,
+                                         w.group_size, _stream()), "unpack_int4")
     _count()
     return codes, scales, zeros
 
@@ -1642,9 +1650,12 @@ def _int4_entry(name: str):
     integers: a few microseconds less than wrapping each)."""
     fn = _INT4_ENTRIES.get(name)
     if fn is None:
-        p, i = ctypes.c_void_p, ctypes.c_int
+        p, i, q = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong
         fn = getattr(_lib(), name)
-        fn.argtypes = {"ix_int4_stream": [p, p, i, p, p, p, i, i, i, i, i, i, p, i, p],
+        fn.argtypes = {"ix_int4_quantize": [p, i, p, q, i, i, i, p],
+                       "ix_int4_pack": [p, p, p, p, q, i, i, i, p],
+                       "ix_int4_unpack": [p, p, p, p, q, i, i, i, p],
+                       "ix_int4_stream": [p, p, i, p, p, p, i, i, i, i, i, i, p, i, p],
                        "ix_int4_tc": [p, p, i, p, p, p, i, i, i, p, i, p, p],
                        "ix_int4_tc_scratch": [p, i, i, i, i]}[name]
         if name == "ix_int4_tc_scratch":
@@ -1695,7 +1706,7 @@ def _int4_stream(what, x, rows, offsets, w, num_rows, out_dtype, rows_per_pass, 
         at = x.data_ptr()
     out = x.new_empty((num_rows, w.cols), dtype=out_dtype)
     _check(_int4_entry("ix_int4_stream")(
-        w._at, at, _dtype_code(x), _at(rows), _at(offsets), out.data_ptr(),
+        w.at, at, _dtype_code(x), _at(rows), _at(offsets), out.data_ptr(),
         1 if out_dtype is torch.float32 else 0, num_rows, x.shape[1], rows_per_pass, active,
         1 if offsets_settled else 0, _at(row_scale), _ACTIVATIONS[activation], _stream()), what)
     _count()
@@ -1713,11 +1724,11 @@ def _int4_tc(what, x, rows, offsets, w, num_rows, out_dtype, row_scale=None, act
     elif rows is not None:
         x = gather_rows(x, rows)
     out = torch.empty((num_rows, w.cols), dtype=out_dtype, device=x.device)
-    need = _int4_entry("ix_int4_tc_scratch")(w._at, num_rows, x.shape[-1],
+    need = _int4_entry("ix_int4_tc_scratch")(w.at, num_rows, x.shape[-1],
                                              0 if offsets is None else 1, terms)
     part = torch.empty(need, dtype=torch.float32, device=x.device) if need else None
     _check(_int4_entry("ix_int4_tc")(
-        w._at, x.data_ptr(), terms, _at(offsets), out.data_ptr(), _at(part),
+        w.at, x.data_ptr(), terms, _at(offsets), out.data_ptr(), _at(part),
         1 if out_dtype is torch.float32 else 0, num_rows, x.shape[-1], _at(row_scale),
         _ACTIVATIONS[activation], _tc_status(x.device).data_ptr(), _stream()), what)
     _count()
