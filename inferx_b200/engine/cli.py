@@ -10,7 +10,8 @@ Option names and meanings follow the reference's ``inferx-serve``
 (``--max-running``, ``--max-seq-len``, ``--kv-blocks``, ``--no-cuda-graphs``).  Options of
 the reference for what this engine does not have are taken only at the value that means
 "off" and refused otherwise, with the reason (``--enable-prefix-caching``,
-``--tensor-parallel-size``, ``--quantization``, ``--kv-cache-dtype``, ``--device``);
+``--tensor-parallel-size``, ``--quantization`` other than ``int4``, ``--kv-cache-dtype``,
+``--device``);
 ``--no-enable-chunked-prefill`` is refused as it is there (options.cc:306-308).
 There is no tokenizer here, so prompts are lists of token ids.
 """
@@ -54,7 +55,10 @@ def build_parser() -> argparse.ArgumentParser:
     ap.add_argument("--no-enable-prefix-caching", dest="prefix_caching", action="store_false")
     ap.add_argument("--tensor-parallel-size", type=int, default=1)
     ap.add_argument("--device", default="cuda")
-    ap.add_argument("--quantization", "-q", default=None)
+    ap.add_argument("--quantization", "-q", default=None,
+                    help="int4: projections, feed-forwards and experts are held in four bits")
+    ap.add_argument("--quantization-group", type=int, default=128, choices=[32, 64, 128],
+                    help="entries of a matrix's row that share a scale and a zero point")
     ap.add_argument("--kv-cache-dtype", default="auto")
     ap.add_argument("--log-level", default="info", choices=["debug", "info", "warning", "error"])
     ap.add_argument("--v", type=int, default=0, help="more detail in debug messages")
@@ -122,8 +126,8 @@ def _refusals(args) -> List[str]:
         why.append("--tensor-parallel-size: this engine runs on one GPU")
     if args.device != "cuda":
         why.append(f"--device {args.device}: this engine runs on CUDA only")
-    if args.quantization not in (None, "none"):
-        why.append("--quantization: weights are bfloat16 or float32 here")
+    if args.quantization not in (None, "none", "int4"):
+        why.append("--quantization: weights are bfloat16 or float32 here, or in four bits with int4")
     if args.kv_cache_dtype not in ("auto", "bfloat16"):
         why.append("--kv-cache-dtype: the cache has the model's element type here")
     return why
@@ -172,7 +176,8 @@ def main(argv=None) -> int:
         num_gpu_blocks_override=args.num_gpu_blocks_override,
         kv_cache_memory_bytes=args.kv_cache_memory_bytes,
         gpu_memory_utilization=args.gpu_memory_utilization, prefill_chunk=args.prefill_chunk,
-        enforce_eager=args.enforce_eager, config_json=cfg_json, seed=args.seed))
+        enforce_eager=args.enforce_eager, config_json=cfg_json, seed=args.seed,
+        quantization=args.quantization, quantization_group=args.quantization_group))
     log("info", f"model ready in {time.time() - t0:.1f}s",
         cache_pages=engine.stats()["pages_total"], page_tokens=args.block_size)
     if args.v > 0:

@@ -40,10 +40,23 @@ class EngineConfig:
     gpu_memory_utilization: float = 0.92   # else this share of the device
     prefill_chunk: int = 0                 # per-prompt tokens per step; 0 = the budget only
     enforce_eager: bool = False            # no CUDA graphs for decode steps
+    quantization: Optional[str] = None     # "int4": matrices are held in four bits
+    quantization_group: int = 128          # entries that share a scale: 32, 64 or 128
     device: str = "cuda"
     # random weights instead of a folder: the config and a seed
     config_json: Optional[Mapping[str, Any]] = None
     seed: int = 0
+
+    def int4_group(self) -> int:
+        """Entries a scale, or 0 where weights keep the run's element type."""
+        if self.quantization in (None, "none"):
+            return 0
+        if self.quantization != "int4":
+            raise ValueError(f"quantization {self.quantization!r} is not one of none, int4")
+        if self.quantization_group not in (32, 64, 128):
+            raise ValueError(f"quantization_group {self.quantization_group} is not one of "
+                             "32, 64, 128")
+        return self.quantization_group
 
     def batched_tokens(self) -> int:
         return self.max_num_batched_tokens or max(2048, self.max_model_len)
@@ -143,14 +156,15 @@ class Engine:
     @classmethod
     def create(cls, config: EngineConfig, ops=None) -> "Engine":
         parse_dtype(config.dtype)
+        int4_group = config.int4_group()
         if config.model is not None:
             mcfg, model = load_model(config.model, dtype=config.dtype, device=config.device,
-                                     ops=ops)
+                                     ops=ops, int4_group=int4_group)
         elif config.config_json is not None:
             mcfg, model = load_model(dtype=config.dtype, device=config.device,
                                      config_json=config.config_json,
                                      source=RandomSource(config.seed, device=config.device),
-                                     ops=ops)
+                                     ops=ops, int4_group=int4_group)
         else:
             raise ValueError("EngineConfig needs a model folder, or a config for random weights")
         pages = autosize_pages(config, model, config.device)

@@ -43,8 +43,10 @@ def pages_for(max_tokens: int, page_size: int, max_live: int = 1) -> int:
 
 class ReplaySession:
     def __init__(self, model_dir: str, dtype: str, max_tokens: int, *, page_size: int = 16,
-                 max_live: int = 8, device: str = "cuda", ops=None, use_graphs: bool = False):
-        _, model = load_model(model_dir, dtype=dtype, device=device, ops=ops)
+                 max_live: int = 8, device: str = "cuda", ops=None, use_graphs: bool = False,
+                 int4_group: int = 0):
+        _, model = load_model(model_dir, dtype=dtype, device=device, ops=ops,
+                              int4_group=int4_group)
         self.runtime = Runtime(model, page_size=page_size,
                                num_pages=pages_for(max_tokens, page_size, max_live),
                                max_slots=max_live,
@@ -133,6 +135,8 @@ def main(argv=None) -> int:
                     help="most tokens live requests hold at any time (each rounded up to 64)")
     ap.add_argument("--block-size", type=int, default=16, help="tokens per cache page")
     ap.add_argument("--max-live", type=int, default=4, help="requests alive at once")
+    ap.add_argument("--int4-group", type=int, default=0, choices=[0, 32, 64, 128],
+                    help="hold matrices in four bits with a scale for so many entries")
     ap.add_argument("--index", action="store_true",
                     help="also write <step>.rows.json: request id and position of each row")
     args = ap.parse_args(argv)
@@ -140,7 +144,7 @@ def main(argv=None) -> int:
         print("trace_run: no CUDA device; this engine has no CPU path", file=sys.stderr)
         return 3
     session = ReplaySession(args.model, args.dtype, args.max_tokens, page_size=args.block_size,
-                            max_live=args.max_live)
+                            max_live=args.max_live, int4_group=args.int4_group)
 
     def report(step):
         sys.stdout.write(f"done {step}\n")

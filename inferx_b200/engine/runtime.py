@@ -43,8 +43,10 @@ def _kernel_ops():
 
 def load_model(model_dir: Optional[str] = None, *, dtype="bfloat16", device="cuda",
                config_json: Optional[Mapping[str, Any]] = None,
-               source: Optional[WeightSource] = None, ops=None):
-    """(typed config, DecoderModel with weights bound).
+               source: Optional[WeightSource] = None, ops=None, int4_group: int = 0):
+    """(typed config, DecoderModel with weights bound).  ``int4_group`` > 0: the matrices that
+    the parts name (projections of attention, feed-forwards, experts) are held in four bits
+    with a scale for so many entries; embedding, head, router, norms and biases are not.
 
     Either ``model_dir`` (config.json + safetensors) or ``config_json`` with a
     ``source`` (for instance a ``RandomSource`` on the device)."""
@@ -60,7 +62,8 @@ def load_model(model_dir: Optional[str] = None, *, dtype="bfloat16", device="cud
         cfg, spec = config_from_json(config_json)
         where = "weights"
         src = source
-    ctx = BuildContext(dtype=run_dtype, device=dev, ops=ops or _kernel_ops())
+    ctx = BuildContext(dtype=run_dtype, device=dev, ops=ops or _kernel_ops(),
+                       int4_group=int4_group)
     model = DecoderModel(spec, ctx)
     model.load(src, where)
     if isinstance(src, CheckpointSource) and source is None:

@@ -1868,6 +1868,8 @@ def gate_up_glu_clamped(x: torch.Tensor, w_gate_up: torch.Tensor, limit: float, 
                         up_shift: float):
     """Front half of a clamped-GLU feed-forward: the fused gate|up product and the
     activation; one weight-streaming kernel for a few rows."""
+    if isinstance(w_gate_up, Int4Weight):
+        return glu_clamped(linear(x, w_gate_up), limit, alpha, up_shift)
     _chk("x", x)
     _chk("w_gate_up", w_gate_up, x.dtype)
     M = x.shape[0]

@@ -25,6 +25,7 @@ class AttentionMixer:
     """Grouped-query attention.  The value heads may have a size of their own
     (``spec.value_dim``): the value pages are then that wide and the fp32-arithmetic
     kernels run; they also run when the spec asks for 32-bit softmax weights."""
+    int4_weights = {"qkv_w": 1, "o_w": 1}
 
     def __init__(self, spec, ctx, prefix: str):
         self.spec = spec
@@ -150,6 +151,7 @@ class TiedKvAttentionMixer:
     keys (both in pages of the same shape, so every paged attention kernel serves), the
     normed queries take the position's temperature, and the scores may be squashed by
     tanh.  Norms, temperature and the squashing are fp32."""
+    int4_weights = {"qk_w": 1, "o_w": 1}
 
     def __init__(self, spec, ctx, prefix: str):
         self.spec, self.ctx, self.prefix = spec, ctx, prefix
@@ -214,6 +216,7 @@ class PreparedAttentionMixer:
     project queries alone and read another layer's keys and values.  Keys and values live in
     the framework's pages (the value pages as wide as the value heads); the convolutions' last
     inputs in the state slots.  Norms, angles, scores and weights are fp32 in every element type."""
+    int4_weights = {"qkv_w": 1, "o_w": 1}
 
     def __init__(self, spec, ctx, prefix: str):
         self.spec, self.ctx, self.prefix = spec, ctx, prefix

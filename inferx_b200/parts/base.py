@@ -24,6 +24,12 @@ Interfaces (duck-typed; a part defined outside this package works the same):
 A part may also define ``check_limits()``; it is called when the model is built and
 raises if a size is beyond what the kernels take, so that a model that cannot run is
 refused before any weight is read rather than at its first launch.
+
+A part whose matrices go through ``ops.linear`` and the gated and grouped products alone may
+name them in ``int4_weights`` (attribute -> 1, or 2 where the rows are a gate matrix and an up
+matrix): where the context asks for it, they are held in four bits once the part is bound.
+A part that is made of parts names those in ``int4_parts`` and may define
+``int4_weights_held()``, called when that is done.
 """
 from __future__ import annotations
 
@@ -38,6 +44,21 @@ class BuildContext:
     dtype: torch.dtype          # element type of activations and matrices
     device: torch.device
     ops: Any                    # the kernel module (inferx_b200.kernels.ops)
+    int4_group: int = 0         # entries a scale where matrices are held in four bits, or 0
+
+
+def hold_in_int4(part, ctx: BuildContext) -> None:
+    """A bound part's matrices in four bits, where it names them and the context asks for it."""
+    if not ctx.int4_group or part is None:
+        return
+    for name, halves in getattr(part, "int4_weights", {}).items():
+        w = getattr(part, name)
+        if isinstance(w, torch.Tensor):
+            setattr(part, name, ctx.ops.quantize_int4(w.contiguous(), ctx.int4_group, halves))
+    for name in getattr(part, "int4_parts", ()):
+        hold_in_int4(getattr(part, name), ctx)
+    if hasattr(part, "int4_weights_held"):
+        part.int4_weights_held()
 
 
 @dataclass(frozen=True)

@@ -18,7 +18,7 @@ import torch
 
 from ..weights import loader as wl
 from ..weights.loader import TensorDecl
-from .base import BuildContext, LayerCache, PendingSum, StepContext
+from .base import BuildContext, LayerCache, PendingSum, StepContext, hold_in_int4
 from .registry import build_part, register_part
 from .streams import read_streams
 
@@ -254,6 +254,7 @@ class DecoderModel:
         for b in self.blocks:
             for part in b.parts():
                 part.bind(fetch(part.tensors()))
+                hold_in_int4(part, self.ctx)
         self.final_norm.bind(fetch(self.final_norm.tensors()))
         if self.embedding is not None:
             self.embedding.bind(fetch(self.embedding.tensors()))

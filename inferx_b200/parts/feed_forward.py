@@ -23,6 +23,8 @@ from .registry import build_part, register_part
 
 
 class SwiGluFeedForward:
+    int4_weights = {"gate_up_w": 2, "down_w": 1}
+
     def __init__(self, spec, ctx, prefix: str):
         self.spec, self.ctx, self.prefix = spec, ctx, prefix
         self.gate_up_w = self.down_w = None
@@ -56,6 +58,7 @@ class ClampedGluFeedForward:
     gated unit whose gate is cut off above and whose linear branch is cut off on both
     sides before one is added to it.  Gate and up are one product over concatenated
     weights; the result leaves in fp32 for the norm that follows."""
+    int4_weights = {"gate_up_w": 1, "down_w": 1}
 
     def __init__(self, spec, ctx, prefix: str):
         self.spec, self.ctx, self.prefix = spec, ctx, prefix
@@ -88,6 +91,7 @@ class BiasedGluFeedForward:
     are one product over concatenated weights; their biases and the activation are one
     pass over its result; the last bias travels with the output as the vector of a pending
     sum, so the norm that adds the output to the stream adds it in the same pass."""
+    int4_weights = {"gate_up_w": 1, "down_w": 1}
 
     def __init__(self, spec, ctx, prefix: str):
         self.spec, self.ctx, self.prefix = spec, ctx, prefix
@@ -136,6 +140,19 @@ _SIDE_STREAMS: dict = {}
 
 
 class MoeFeedForward:
+    int4_parts = ("shared",)
+
+    @property
+    def int4_weights(self):
+        # (experts without a gate have one matrix on the way up)
+        return {"expert_gate_up": 1 if self.activation else 2, "expert_down": 1}
+
+    def int4_weights_held(self):
+        if self.shared is not None:
+            held = [getattr(self.shared, n) for n in getattr(self.shared, "int4_weights", {})]
+            if held:
+                self._shared_bytes = sum(w.nbytes for w in held)
+
     def __init__(self, spec, ctx, prefix: str):
         self.spec, self.ctx, self.prefix = spec, ctx, prefix
         self.identity = int(getattr(spec, "identity_experts", 0) or 0)
@@ -367,6 +384,7 @@ class MoeFeedForward:
 class ReluSquaredFeedForward:
     """``down(relu(up h)^2)``, no biases; the result leaves in fp32 for the norm that adds
     it."""
+    int4_weights = {"up_w": 1, "down_w": 1}
 
     def __init__(self, spec, ctx, prefix: str):
         self.spec, self.ctx, self.prefix = spec, ctx, prefix
@@ -391,6 +409,7 @@ class ReluSquaredFeedForward:
 class ActivatedMlpFeedForward:
     """``down(act(up h))``, no biases; the activation sits in the product's epilogue where the
     step is small enough for this library's own kernels."""
+    int4_weights = {"up_w": 1, "down_w": 1}
 
     def __init__(self, spec, ctx, prefix: str):
         self.spec, self.ctx, self.prefix = spec, ctx, prefix
@@ -419,6 +438,7 @@ class TableMoeFeedForward:
     the look-up it is the routed mixture's own path: stable dispatch by expert, grouped
     gate/up product with silu(gate) * up, grouped down product, combine in slot order with
     fp32 weights."""
+    int4_weights = {"expert_gate_up": 2, "expert_down": 1}
 
     def __init__(self, spec, ctx, prefix: str):
         self.spec, self.ctx, self.prefix = spec, ctx, prefix

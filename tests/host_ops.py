@@ -66,6 +66,9 @@ class HostInt4:
     def to(self, dtype):
         return self.dense(dtype)
 
+    def contiguous(self):
+        return self
+
     def __getitem__(self, e):
         return HostInt4(self.codes[e], self.scales[e], self.zeros[e], self.group_size, self.halves)
 
