@@ -19,8 +19,9 @@
 //   2      brings the codes and parameters of the block's eight strips (one bulk copy, DUAL two);
 //   4-11   take each finished group's sums out of tensor memory, a weight row a lane, add scale * sum to
 //          fp32 registers, and leave an item's results in shared memory;
-//   12-19  unpack a strip each: a lane's sixteen bytes of codes, less their zero points, are whole numbers
-//          that lie in registers as tensor memory wants them (16 rows by 256 bits);
+//   12-19  unpack, four the even chunks and four the odd ones, two strips a warp: a lane's sixteen bytes
+//          of codes, less their zero points, are whole numbers that lie in registers as tensor memory
+//          wants them (16 rows by 256 bits);
 //   20-23  finish and store the results of an item while the next one is under way.
 // Rows of a DUAL item lie as 16 gate rows, the 16 up rows of the same columns, and so on.
 // So the operands of the tensor cores are exact (a code less its zero point has five bits), the sums of
@@ -125,6 +126,17 @@ __device__ __forceinline__ bool i4t_wait(unsigned long long* bar, unsigned parit
   }
   return false;
 }
+// One lane of the warp, known to the compiler to be one: with `lane == 0` the eight MMAs of a chunk
+// take 700 cycles to issue, with this 250.
+__device__ __forceinline__ bool i4t_elect() {
+  unsigned ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok));
+  return ok != 0;
+}
 // The pair's MMA with the weights in tensor memory (each block's rows in its own).
 __device__ __forceinline__ void i4t_mma(unsigned d, unsigned a, unsigned long long bdesc,
                                         unsigned idesc, unsigned accum) {
@@ -210,7 +222,7 @@ int4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
   float* stage = reinterpret_cast<float*>(xs + C::X_RING * C::X_STAGE);   // [row of the tile][128]
   unsigned char* cs = reinterpret_cast<unsigned char*>(stage + BT * 128);
   unsigned short* scales = reinterpret_cast<unsigned short*>(cs + C::C_RING * 8 * C::C_BYTES);
-  // A group may be multiplied: on a chunk's first group the block's operands are there (eight unpacking
+  // A group may be multiplied: on a chunk's first group the block's operands are there (four unpacking
   // warps and the rows' bytes), an accumulator's sums are taken (eight warps), and, in the first block,
   // the second one is as far.  One barrier for all of it, as a wait costs the issuing warp hundreds of
   // cycles even where nothing is waited for.
@@ -250,13 +262,13 @@ int4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
   }
   if (threadIdx.x == 0) {
     for (int s = 0; s < I4T_DONE; ++s)
-      for (int q = 0; q < NG; ++q) mbar_init(&go[s][q], (q == 0 ? 17 : 8) + (rank == 0 ? 1 : 0));
+      for (int q = 0; q < NG; ++q) mbar_init(&go[s][q], (q == 0 ? 13 : 8) + (rank == 0 ? 1 : 0));
     for (int s = 0; s < C::C_RING; ++s) {
       mbar_init(&full_c[s], 1);
-      mbar_init(&empty_c[s], 8);
+      mbar_init(&empty_c[s], 4);
     }
     for (int s = 0; s < I4T_DONE; ++s) mbar_init(&done[s], 1);
-    for (int s = 0; s < C::S_RING; ++s) mbar_init(&full_s[s], 8);
+    for (int s = 0; s < C::S_RING; ++s) mbar_init(&full_s[s], 4);
     for (int b = 0; b < 2; ++b) mbar_init(&acc_full[b], 1);
     mbar_init(&stage_full, 8);
     mbar_init(&stage_empty, 4);
@@ -373,13 +385,13 @@ int4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
             tc_fence_after();
             if (rank != 0) {
               tc_fence_before();
-              if (lane == 0) i4t_arrive_at(first_block + (slot * NG + q) * 8);
+              if (i4t_elect()) i4t_arrive_at(first_block + (slot * NG + q) * 8);
               __syncwarp();
               continue;
             }
             const int buf = group & 1;
             const unsigned sums = tmem_base + buf * BT;
-            if (lane == 0) {
+            if (i4t_elect()) {
 #pragma unroll
               for (int i = 0; i < GROUP / 16; ++i) {
                 // sixteens of k into the chunk: eight columns of weights, 32 bytes of a row
@@ -519,59 +531,78 @@ int4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
     if (!ok && lane == 0 && !*abortp) { atomicExch(p.status, I4T_ERR_STORE); *abortp = 1; }
   } else if (warp >= 12) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    // its strip: one that the warp's lanes of tensor memory hold
-    const int unpacker = 2 * (warp & 3) + ((warp - 12) >> 2);
+    // its strips: the two that the warp's lanes of tensor memory hold
+    const int quarter = warp & 3, turn = (warp - 12) >> 2;
     const int g = lane >> 2, t = lane & 3;
-    const unsigned to = tmem_base + 2 * BT + ((unsigned)(unpacker * 16) << 16);
-    // (DUAL: four gate strips were copied, then four up strips)
-    const int from = DUAL ? (unpacker & 1) * 4 + (unpacker >> 1) : unpacker;
+    const unsigned to = tmem_base + 2 * BT + ((unsigned)(quarter * 32) << 16);
     int n = 0;
     bool ok = true;
     for (int w = first; w < n_items && ok; w += step) {
       const I4TItem it = item_of(w);
       if (it.n <= 0) continue;
-      for (int c = it.c0; c < it.c1; ++c, ++n) {
+      const int chunks = it.c1 - it.c0, end = n + chunks;
+      for (n += (n & 1) != turn; n < end; n += 2) {
         const int sc = n % C::C_RING, sa = n % C::A_RING;
         ok = wait(&full_c[sc], n / C::C_RING & 1);
         if (!ok) break;
-        const unsigned* own = reinterpret_cast<const unsigned*>(cs + (sc * 8 + from) * C::C_BYTES);
-        uint4 code[2];
-        unsigned pa[NG], pb[NG];
-        code[0] = *reinterpret_cast<const uint4*>(own + lane * 4);
-        code[1] = *reinterpret_cast<const uint4*>(own + I4_TILE_WORDS + lane * 4);
+        // (DUAL: four gate strips were copied, then four up strips)
+        const unsigned* own[2];
+        uint4 code[2][2];
 #pragma unroll
-        for (int i = 0; i < NG; ++i) {
-          pa[i] = own[I4_CODE_WORDS + g * NG + i];
-          pb[i] = own[I4_CODE_WORDS + (g + 8) * NG + i];
+        for (int i = 0; i < 2; ++i) {
+          own[i] = reinterpret_cast<const unsigned*>(
+              cs + (sc * 8 + (DUAL ? i * 4 + quarter : 2 * quarter + i)) * C::C_BYTES);
+          code[i][0] = *reinterpret_cast<const uint4*>(own[i] + lane * 4);
+          code[i][1] = *reinterpret_cast<const uint4*>(own[i] + I4_TILE_WORDS + lane * 4);
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&empty_c[sc]);
+        // (parameters of groups of 64 or 32 are read when their strip's turn comes: there are not the
+        // registers to hold them all)
+        unsigned pa[2][NG], pb[2][NG];
+        auto params = [&](int i) {
+#pragma unroll
+          for (int j = 0; j < NG; ++j) {
+            pa[i][j] = own[i][I4_CODE_WORDS + g * NG + j];
+            pb[i][j] = own[i][I4_CODE_WORDS + (g + 8) * NG + j];
+          }
+          if (i == 1) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&empty_c[sc]);
+          }
+        };
+        if (NG == 1) {
+          params(0);
+          params(1);
+        }
         if (n >= C::A_RING) {
           const int before = n - C::A_RING;
           ok = wait(&done[before % I4T_DONE], before / I4T_DONE & 1);
           if (!ok) break;
         }
-        // the scales, by row and group, to the warps that add up
-        if (t == 0) {
-          unsigned short* to = scales + ((n % C::S_RING) * 128 + unpacker * 16 + g) * NG;
-          i4t_scales<NG>(to, pa);
-          i4t_scales<NG>(to + 8 * NG, pb);
-        }
         tc_fence_after();
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const unsigned word[4] = {code[h].x, code[h].y, code[h].z, code[h].w};
-          unsigned v[16];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int group = (h * 4 + j) * 16 / GROUP;
-            const unsigned sa2 = i4_sub(pa[group]), sb2 = i4_sub(pb[group]);
-            v[4 * j] = i4_pair(word[j], 0, sa2);
-            v[4 * j + 1] = i4_pair(word[j], 2, sa2);
-            v[4 * j + 2] = i4_pair(word[j], 1, sb2);
-            v[4 * j + 3] = i4_pair(word[j], 3, sb2);
+        for (int i = 0; i < 2; ++i) {
+          if (NG > 1) params(i);
+          // the scales, by row and group, to the warps that add up
+          if (t == 0) {
+            unsigned short* row = scales + ((n % C::S_RING) * 128 + quarter * 32 + i * 16 + g) * NG;
+            i4t_scales<NG>(row, pa[i]);
+            i4t_scales<NG>(row + 8 * NG, pb[i]);
           }
-          i4t_put(to + sa * 64 + h * 32, v);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const unsigned word[4] = {code[i][h].x, code[i][h].y, code[i][h].z, code[i][h].w};
+            unsigned v[16];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int group = (h * 4 + j) * 16 / GROUP;
+              const unsigned sa2 = i4_sub(pa[i][group]), sb2 = i4_sub(pb[i][group]);
+              v[4 * j] = i4_pair(word[j], 0, sa2);
+              v[4 * j + 1] = i4_pair(word[j], 2, sa2);
+              v[4 * j + 2] = i4_pair(word[j], 1, sb2);
+              v[4 * j + 3] = i4_pair(word[j], 3, sb2);
+            }
+            i4t_put(to + ((unsigned)(i * 16) << 16) + sa * 64 + h * 32, v);
+          }
         }
         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         tc_fence_before();
@@ -581,6 +612,7 @@ int4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
           mbar_arrive(&full_s[n % C::S_RING]);
         }
       }
+      n = end;
     }
     if (!ok && lane == 0 && !*abortp) { atomicExch(p.status, I4T_ERR_UNPACK); *abortp = 1; }
   } else {
@@ -753,9 +785,15 @@ static I4TPlan i4t_plan(int rows, int N, int Kp, int E, bool grouped, bool dual,
     for (int splits = 1; splits <= (rows > 4096 ? 1 : 16) && splits <= chunks; ++splits) {
       const int run = (chunks + splits - 1) / splits;
       if ((long long)run * (splits - 1) >= chunks) continue;      // an empty last run
+      // Least squares over 166 timed cuts of eight products, each in both types (64 to 2,048 rows, 2 to
+      // 37 MB of codes): half of them off by 5 % at most, eight in ten by 9 %, and the cut with the
+      // lowest estimate was the fastest of those timed for every one of the sixteen.
       const long long items = (long long)((rows + per - 1) / per) * f_tiles * splits;
-      const double us = (double)((items + pairs - 1) / pairs) * (run * (0.25 + 0.0015 * terms * per) + 1.5) +
-                        (splits > 1 ? 2.0 + splits * (double)rows * N * (dual ? 2 : 1) * 1.6e-6 : 0.0);
+      const double waves = (double)((items + pairs - 1) / pairs);
+      const double chunk = terms == 3 ? 0.55 + 0.0058 * per : 0.40 + 0.0017 * per;
+      const double join = (terms == 3 ? 0.55 : 0.34) * 4e-6 * splits * (double)rows * N * (dual ? 2 : 1);
+      const double us = waves * (run * chunk + (terms == 3 ? 0.1 : 1.1)) + 6.0 +
+                        (splits > 1 ? 3.4 + join : 0.0);
       if (best < 0 || us < 0.98 * best) {
         best = us;
         plan.tile_rows = per;
