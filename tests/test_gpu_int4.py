@@ -24,6 +24,18 @@ def ops():
     return o
 
 
+@pytest.fixture(params=["chosen", "few rows", "many rows"])
+def kernel(request, monkeypatch):
+    """The products as the rules choose their kernel, and each kernel for calls of either's sizes."""
+    if request.param != "chosen":
+        most = 0 if request.param == "many rows" else 1 << 62
+        each = {torch.bfloat16: most, torch.float32: most}
+        monkeypatch.setattr(ops(), "INT4_STREAM_ROWS", most)
+        monkeypatch.setattr(ops(), "INT4_STREAM_ROW_BYTES", each)
+        monkeypatch.setattr(ops(), "INT4_STREAM_ROWS_PER_EXPERT", each)
+    return request.param
+
+
 def gen(seed):
     g = torch.Generator(device="cuda")
     g.manual_seed(seed)
@@ -130,6 +142,7 @@ SIZES = [(1, 1, 1), (1, 128, 16), (2, 40, 15), (3, 129, 17), (7, 1000, 515), (8,
          (64, 2048, 130), (65, 72, 256), (130, 520, 129), (257, 1408, 300), (1, 20480, 48)]
 
 
+@pytest.mark.usefixtures("kernel")
 @pytest.mark.parametrize("dtype,out", [(torch.bfloat16, torch.bfloat16),
                                        (torch.bfloat16, torch.float32),
                                        (torch.float32, torch.float32)])
@@ -147,6 +160,7 @@ def test_linear(dtype, out, group, m, k, n):
     assert torch.equal(got, ops().linear(x, q, out_dtype=out))
 
 
+@pytest.mark.usefixtures("kernel")
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("group", [32, 64, 128])
 @pytest.mark.parametrize("m,k,n", [(1, 128, 16), (2, 40, 15), (8, 2048, 88), (13, 333, 65),
@@ -161,6 +175,7 @@ def test_gated(dtype, group, m, k, n):
     near(got, *gated(x, w.dense(torch.float64)))
 
 
+@pytest.mark.usefixtures("kernel")
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("activation", ["gelu", "relu_squared"])
 @pytest.mark.parametrize("m", [3, 150])
@@ -180,6 +195,7 @@ def test_linear_act(dtype, activation, m):
         near(got, y.clamp(min=0) ** 2, 2 * y.abs() * d + d * d + y * y * 2.0 ** -23)
 
 
+@pytest.mark.usefixtures("kernel")
 @pytest.mark.parametrize("m", [2, 40, 200])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_infinities_and_nan_stay_in_their_rows(m, dtype):
@@ -199,6 +215,7 @@ def test_infinities_and_nan_stay_in_their_rows(m, dtype):
     assert torch.equal(got[0].double()[~torch.isnan(want[0])], want[0][~torch.isnan(want[0])])
 
 
+@pytest.mark.usefixtures("kernel")
 def test_weights_that_hold_an_infinity_say_so():
     w = matrix((40, 256), gen(6), torch.bfloat16)
     w[7, 130] = float("inf")
@@ -209,6 +226,7 @@ def test_weights_that_hold_an_infinity_say_so():
         assert torch.isfinite(y[:, 8:]).all()
 
 
+@pytest.mark.usefixtures("kernel")
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_great_and_small_activations_keep_their_bits(dtype):
     """Rows scaled by powers of two give results scaled by them, bit for bit."""
@@ -224,6 +242,7 @@ def test_great_and_small_activations_keep_their_bits(dtype):
         assert torch.equal(y[3], y[0] * 2.0 ** 100)
 
 
+@pytest.mark.usefixtures("kernel")
 def test_misaligned_rows():
     """A contiguous view that starts in the middle of a buffer."""
     g = gen(9)
@@ -234,6 +253,7 @@ def test_misaligned_rows():
         assert torch.equal(ops().linear(x, q), ops().linear(x.clone(), q))
 
 
+@pytest.mark.usefixtures("kernel")
 def test_no_rows():
     q = ops().quantize_int4(matrix((50, 64), gen(1)), 32)
     y = ops().linear(torch.empty((0, 64), device="cuda"), q)
@@ -251,6 +271,7 @@ def routed(tokens, experts, top, g, skew=0.0):
     return (order // top).to(torch.int32), offsets
 
 
+@pytest.mark.usefixtures("kernel")
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("group", [32, 64, 128])
 @pytest.mark.parametrize("tokens,experts,top,hidden,inner,skew", [
@@ -279,6 +300,7 @@ def test_experts_up_and_down(dtype, group, tokens, experts, top, hidden, inner, 
             near(y[a:b], act[a:b].double() @ w.t(), sums_error(act[a:b], w))
 
 
+@pytest.mark.usefixtures("kernel")
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("tokens", [2, 90])
 def test_experts_without_a_gate(dtype, tokens):
@@ -296,6 +318,7 @@ def test_experts_without_a_gate(dtype, tokens):
         near(got[a:b], y.clamp(min=0) ** 2, 2 * y.abs() * d + d * d + y * y * 2.0 ** -23)
 
 
+@pytest.mark.usefixtures("kernel")
 def test_rows_behind_the_last_expert_are_left_alone():
     """Rows of experts that are not there (a router's identity outputs) get no product, and
     what stands there does not reach the others."""
@@ -311,7 +334,51 @@ def test_rows_behind_the_last_expert_are_left_alone():
     assert torch.allclose(part[:last].float(), alone.float(), rtol=2.0 ** -7, atol=1e-6)
 
 
+@pytest.mark.usefixtures("kernel")
+@pytest.mark.parametrize("kernel", ["many rows"], indirect=True)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("m,k,n,halves", [
+    (193, 5632, 260, 1),       # runs of K that are joined
+    (2500, 384, 777, 2),       # more tiles than pairs of SMs, a short last one
+    (700, 2048, 2048, 1), (4100, 136, 520, 1), (385, 640, 1409, 2)])
+def test_many_rows(dtype, group, m, k, n, halves):
+    """Tiles of each height, several of them to a pair, more rows than one run of K serves."""
+    g = gen(m + n)
+    q = ops().quantize_int4(matrix((halves * n, k), g), group, halves=halves)
+    codes, scales, zeros = ops().unpack_int4(q)
+    at = torch.arange(k, device="cuda") // group
+    w = scales.double()[:, at] * (codes.double() - zeros.double()[:, at])
+    x = torch.randn((m, k), generator=g, device="cuda").to(dtype)
+    if halves == 2:
+        near(ops().gate_up_swiglu(x, q), *gated(x, w))
+    else:
+        near(ops().linear(x, q), x.double() @ w.t(), sums_error(x, w))
+
+
+@pytest.mark.usefixtures("kernel")
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("experts", [1, 1024, 1030])
+def test_as_many_experts_as_there_may_be(dtype, experts):
+    """The same expert for all rows, with all others empty, and rows that are named twice."""
+    g = gen(experts)
+    w = H.quantize_int4(matrix((experts, 40, 96), g), 32)
+    q = ops().pack_int4(w.codes, w.scales, w.zeros, 32)
+    for here, count in ((0, 37), (experts - 1, 37), (experts // 2, 700)):
+        x = torch.randn((count, 96), generator=g, device="cuda").to(dtype)
+        offsets = torch.zeros(experts + 1, dtype=torch.int32, device="cuda")
+        offsets[here + 1:] = count
+        dense = w[here].dense(torch.float64)
+        near(ops().grouped_down(x, offsets, q), x.double() @ dense.t(), sums_error(x, dense))
+        twice = torch.arange(count, device="cuda", dtype=torch.int32) // 2
+        mine = x[twice.long()]
+        y, d = mine.double() @ dense.t(), sums_error(mine, dense)
+        near(ops().grouped_up(x, twice, offsets, q, "relu_squared"), y.clamp(min=0) ** 2,
+             2 * y.abs() * d + d * d + y * y * 2.0 ** -23)
+
+
 # -- streams, graphs, refusals -----------------------------------------------------------
+@pytest.mark.usefixtures("kernel")
 @pytest.mark.parametrize("m", [4, 120])
 def test_recorded_calls_follow_their_inputs(m):
     g = gen(12)
@@ -337,6 +404,7 @@ def test_recorded_calls_follow_their_inputs(m):
             assert torch.equal(y, want)
 
 
+@pytest.mark.usefixtures("kernel")
 def test_calls_on_two_streams():
     g = gen(13)
     q = ops().quantize_int4(matrix((512, 1024), g), 128)
