@@ -1525,26 +1525,26 @@ class Int4Weight:
     size, which the gated products want, and 1 otherwise.  ``data`` is an int32 tensor in the
     kernels' own layout; ``cols`` counts a product's output columns, the rows of one half."""
 
-    __slots__ = ("shape", "halves", "group_size", "data", "experts", "cols", "inner", "per_expert",
-                 "device_index", "_record", "_at")
+    __slots__ = ("shape", "halves", "group_size", "_data", "experts", "cols", "inner", "per_expert",
+                 "device_index", "_record", "at")
 
     def __init__(self, shape, halves: int, group_size: int, data: torch.Tensor):
         self.shape = torch.Size(shape)
-        self.halves, self.group_size, self.data = halves, group_size, data
+        self.halves, self.group_size, self._data = halves, group_size, data
         self.experts = self.shape[0] if len(self.shape) == 3 else 1
         self.per_expert = len(self.shape) == 3
         self.cols, self.inner = self.shape[-2] // halves, self.shape[-1]
         self.device_index = data.get_device()
-        self._record = None
+        # what a product's entry point reads, and where (made once: threads share a weight)
+        self._record = _Int4Record(data.data_ptr(), self.cols, self.experts, group_size, halves - 1)
+        self.at = ctypes.addressof(self._record)
+
+    def __reduce__(self):
+        return Int4Weight, (self.shape, self.halves, self.group_size, self._data)
 
     @property
-    def at(self) -> int:
-        """Where the record is that a product's entry point reads."""
-        if self._record is None:
-            self._record = _Int4Record(self.data.data_ptr(), self.cols, self.experts,
-                                       self.group_size, self.halves - 1)
-            self._at = ctypes.addressof(self._record)
-        return self._at
+    def data(self) -> torch.Tensor:
+        return self._data
 
     @property
     def device(self):
@@ -1757,7 +1757,7 @@ def _int4_product(what: str, x: torch.Tensor, w: Int4Weight, halves: int,
     if out_dtype not in (torch.float32, x.dtype):
         raise KernelError(f"{what}: results in {out_dtype} from activations in {x.dtype}")
     M = x.shape[0]
-    if M <= INT4_STREAM_ROWS or M * w.data.nbytes <= INT4_STREAM_ROW_BYTES[x.dtype]:
+    if M <= INT4_STREAM_ROWS or M * w._data.nbytes <= INT4_STREAM_ROW_BYTES[x.dtype]:
         if M == 0:
             return torch.empty((0, w.cols), dtype=out_dtype, device=x.device)
         return _int4_stream(what, x, None, None, w, M, out_dtype, M, activation=activation)

@@ -47,18 +47,22 @@ class BuildContext:
     int4_group: int = 0         # entries a scale where matrices are held in four bits, or 0
 
 
-def hold_in_int4(part, ctx: BuildContext) -> None:
-    """A bound part's matrices in four bits, where it names them and the context asks for it."""
+def hold_in_int4(part, ctx: BuildContext) -> int:
+    """A bound part's matrices in four bits, where it names them and the context asks for it;
+    how many that were."""
     if not ctx.int4_group or part is None:
-        return
+        return 0
+    held = 0
     for name, halves in getattr(part, "int4_weights", {}).items():
         w = getattr(part, name)
         if isinstance(w, torch.Tensor):
             setattr(part, name, ctx.ops.quantize_int4(w.contiguous(), ctx.int4_group, halves))
+            held += 1
     for name in getattr(part, "int4_parts", ()):
-        hold_in_int4(getattr(part, name), ctx)
+        held += hold_in_int4(getattr(part, name), ctx)
     if hasattr(part, "int4_weights_held"):
         part.int4_weights_held()
+    return held
 
 
 @dataclass(frozen=True)

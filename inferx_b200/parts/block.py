@@ -251,10 +251,13 @@ class DecoderModel:
         self.stream_tables = {n: t for n, t in own.items()
                               if n not in (self.spec.embed_name, self.spec.head_name)}
         # (the matrices of stream projections live in the same table, by name)
+        matrices = 0
         for b in self.blocks:
             for part in b.parts():
                 part.bind(fetch(part.tensors()))
-                hold_in_int4(part, self.ctx)
+                matrices += hold_in_int4(part, self.ctx)
+        if self.ctx.int4_group and not matrices:
+            raise ValueError("no part of this model names matrices that can be held in four bits")
         self.final_norm.bind(fetch(self.final_norm.tensors()))
         if self.embedding is not None:
             self.embedding.bind(fetch(self.embedding.tensors()))

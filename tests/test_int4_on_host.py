@@ -168,3 +168,27 @@ def test_the_plain_statement_of_quantising():
     assert ((q.dense() - w).abs() <= step * (0.5 + 16 * 2.0 ** -8)).all()
 
 
+
+
+def test_a_weight_keeps_the_tensor_that_its_record_names():
+    import copy
+    import pickle
+    q = kernel_ops._int4_empty("here", (4, 96, 200), 64, 2, "cpu")
+    q.data.random_(-2 ** 31, 2 ** 31 - 1)
+    assert q._record.data == q.data.data_ptr() and q._record.cols == 48
+    with pytest.raises(AttributeError):
+        q.data = q.data.clone()
+    for other in (copy.deepcopy(q), pickle.loads(pickle.dumps(q))):
+        assert other._record.data == other.data.data_ptr() != q.data.data_ptr()
+        assert torch.equal(other.data, q.data) and other.shape == q.shape
+        assert (other.halves, other.group_size, other.cols, other.inner, other.experts) == \
+            (2, 64, 48, 200, 4)
+    assert copy.copy(q).data is q.data
+
+
+def test_a_model_whose_parts_name_no_matrices_is_refused(monkeypatch):
+    from inferx_b200.parts import block
+    monkeypatch.setattr(block, "hold_in_int4", lambda part, ctx: 0)
+    with pytest.raises(ValueError, match="no part of this model"):
+        load_model(config_json=TINY_A, source=RandomSource(1), dtype="float32", device="cpu", ops=H,
+                   int4_group=32)
