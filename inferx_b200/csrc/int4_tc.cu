@@ -28,6 +28,17 @@
 // a group are the tensor cores' fp32, and a group's scale multiplies in fp32: no weight is rounded to
 // bfloat16.
 //
+// Measured (bfloat16, groups of 128): 2,048 rows, 2,048 -> 6,144 57.5 us (897 TFLOP/s); 4,096 rows, 3,584 ->
+// 4,096 111 us (1,085; a bfloat16 library product alone reaches 1,670); gated, 2,048 rows, 2,048 -> 2 x
+// 5,632 96 us (989); 60 experts of 2 x 1,408 x 2,048 with 137 rows each 133 us (710).  What bounds it: a chunk
+// of 192 rows takes 1,330 cycles where its MMAs are 768.  The summing warps need 700 for their 96 columns
+// and 630 more from one accumulator to the next (the arrival, two waits), and an operand stage is full
+// again 1,300 after its MMAs have run; tensor memory has room for two accumulators and two stages.
+// Groups of 64 or 32 have two or four sums a chunk to take: 2,048 -> 6,144 with groups of 64 80.6 us.
+// Built and slower: every warp of the second block arriving at the first's barrier by itself (64 us
+// where the one relay had 60), sixteen columns of sums on their way while sixteen are added (61 against
+// 59), polling barriers instead of sleeping on them (63 against 59).
+//
 // Columns past the tile and weight rows past N are computed on whatever is there and never stored.
 // Every wait on an mbarrier is bounded: the waiter records a code in `status` (51 and 54 copies, 52
 // MMAs, 53 unpacking, 55 sums, 56 results), raises a flag that ends its block's other roles, and the pair meets at
@@ -84,6 +95,7 @@ template <int TERMS, bool DUAL, int BT, int GROUP> struct I4TCfg {
                               S_RING * 128 * (128 / GROUP) * 2 + 1024;
   static_assert(SMEM + 4608 <= 227 * 1024, "shared memory");
   static_assert(X_RING <= I4T_DONE && A_RING <= I4T_DONE, "a stage's last use is still to be seen");
+  static_assert(A_RING % 2 == 0 && S_RING % 2 == 0, "a stage's chunks are the same four warps'");
   static_assert(BT % 64 == 0 && 2 * BT + 64 * A_RING <= 512, "tensor memory");
   static constexpr int F = DUAL ? 128 : 256;                   // output columns of an item
 };
@@ -227,7 +239,11 @@ int4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
   // the second one is as far.  One barrier for all of it, as a wait costs the issuing warp hundreds of
   // cycles even where nothing is waited for.
   __shared__ __align__(8) unsigned long long go[I4T_DONE][NG];
-  __shared__ __align__(8) unsigned long long full_c[C::C_RING], empty_c[C::C_RING];
+  // Codes of a chunk are there.  Two barriers for every stage, chunks in turn, so that a barrier's
+  // chunks are all unpacked by the same four warps: a wait for a phase is only right where the phase
+  // before has been waited for, and with three stages and one barrier each the phase before belongs to
+  // the other four warps, whose copy may land later.
+  __shared__ __align__(8) unsigned long long full_c[2 * C::C_RING], empty_c[C::C_RING];
   __shared__ __align__(8) unsigned long long done[I4T_DONE];     // a chunk's MMAs have run
   __shared__ __align__(8) unsigned long long full_s[C::S_RING];  // a chunk's scales are there
   __shared__ __align__(8) unsigned long long acc_full[2];
@@ -263,10 +279,8 @@ int4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
   if (threadIdx.x == 0) {
     for (int s = 0; s < I4T_DONE; ++s)
       for (int q = 0; q < NG; ++q) mbar_init(&go[s][q], (q == 0 ? 13 : 8) + (rank == 0 ? 1 : 0));
-    for (int s = 0; s < C::C_RING; ++s) {
-      mbar_init(&full_c[s], 1);
-      mbar_init(&empty_c[s], 4);
-    }
+    for (int s = 0; s < 2 * C::C_RING; ++s) mbar_init(&full_c[s], 1);
+    for (int s = 0; s < C::C_RING; ++s) mbar_init(&empty_c[s], 4);
     for (int s = 0; s < I4T_DONE; ++s) mbar_init(&done[s], 1);
     for (int s = 0; s < C::S_RING; ++s) mbar_init(&full_s[s], 4);
     for (int b = 0; b < 2; ++b) mbar_init(&acc_full[b], 1);
@@ -430,10 +444,11 @@ int4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
           if (!ok) break;
           if (lane == 0) {
             unsigned char* to = cs + s * 8 * C::C_BYTES;
-            mbar_expect_tx(&full_c[s], DUAL ? 2 * bytes : bytes);
+            unsigned long long* full = &full_c[n % (2 * C::C_RING)];
+            mbar_expect_tx(full, DUAL ? 2 * bytes : bytes);
             if (bytes) {
-              i4t_copy(to, from, bytes, &full_c[s]);
-              if (DUAL) i4t_copy(to + 4 * C::C_BYTES, from + p.chunks * pitch, bytes, &full_c[s]);
+              i4t_copy(to, from, bytes, full);
+              if (DUAL) i4t_copy(to + 4 * C::C_BYTES, from + p.chunks * pitch, bytes, full);
             }
           }
           __syncwarp();
@@ -442,7 +457,7 @@ int4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
       if (lane == 0) {
         if (!ok && !*abortp) { atomicExch(p.status, I4T_ERR_CODES); *abortp = 1; }
         for (int f = max(0, n - C::C_RING); f < n; ++f)
-          mbar_drain(&full_c[f % C::C_RING], f / C::C_RING & 1);
+          mbar_drain(&full_c[f % (2 * C::C_RING)], f / (2 * C::C_RING) & 1);
       }
     }
   } else if (warp >= 20) {
@@ -543,7 +558,7 @@ int4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
       const int chunks = it.c1 - it.c0, end = n + chunks;
       for (n += (n & 1) != turn; n < end; n += 2) {
         const int sc = n % C::C_RING, sa = n % C::A_RING;
-        ok = wait(&full_c[sc], n / C::C_RING & 1);
+        ok = wait(&full_c[n % (2 * C::C_RING)], n / (2 * C::C_RING) & 1);
         if (!ok) break;
         // (DUAL: four gate strips were copied, then four up strips)
         const unsigned* own[2];

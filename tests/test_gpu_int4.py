@@ -377,6 +377,33 @@ def test_as_many_experts_as_there_may_be(dtype, experts):
              2 * y.abs() * d + d * d + y * y * 2.0 ** -23)
 
 
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("hidden,inner", [(2048, 520), (1408, 264)])
+def test_codes_that_land_out_of_order(group, hidden, inner):
+    """Long prompts over weights that are not in the second-level cache: a chunk's codes may land
+    after the next one's.  Every call gives the same bits, and they are the product's."""
+    g = gen(hidden + group)
+    experts, tokens = 24, 1100
+    rows, offsets = routed(tokens, experts, 4, g, 1.0)
+    q = ops().quantize_int4(matrix((experts, 2 * inner, hidden), g), group, halves=2)
+    x = torch.randn((tokens, hidden), generator=g, device="cuda").to(torch.bfloat16)
+    other = torch.empty(160 << 20, dtype=torch.uint8, device="cuda")
+    first = None
+    for i in range(12):
+        other.fill_(i)
+        got = ops().grouped_gate_up_swiglu(x, rows, offsets, q)
+        first = got if first is None else first
+        assert torch.equal(got, first)
+    ops().check_async_errors()
+    codes, scales, zeros = ops().unpack_int4(q)
+    at = torch.arange(hidden, device="cuda") // group
+    bounds = offsets.tolist()
+    for e in (0, 7, experts - 1):
+        w = scales[e].double()[:, at] * (codes[e].double() - zeros[e].double()[:, at])
+        a, b = bounds[e], bounds[e + 1]
+        near(first[a:b], *gated(x[rows[a:b].long()], w))
+
+
 # -- streams, graphs, refusals -----------------------------------------------------------
 @pytest.mark.usefixtures("kernel")
 @pytest.mark.parametrize("m", [4, 120])
