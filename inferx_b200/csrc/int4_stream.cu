@@ -18,9 +18,9 @@
 // ones summed apart from the first.  The warps of a block split K by chunks and join their sums through
 // shared memory in warp order, so a row's result does not depend on which rows share its tile.
 //
-// Measured (bfloat16, groups of 128; us, GB/s of codes and parameters): one row, 2,048 -> 2,048 2.9 (760);
-// eight rows, 5,632 -> 2,048 4.7 (1,300); eight rows gated, 3,584 -> 2 x 20,480 28 (2,800); eight tokens of 4 of
-// 60 experts of 2 x 1,408 x 2,048 31.5 up and 15.9 down (2,500).  The short ones are a chain of latencies
+// Measured (bfloat16, groups of 128; us, GB/s of codes): one row, 2,048 -> 2,048 2.9 (725); eight rows,
+// 5,632 -> 2,048 5.0 (1,140); eight rows gated, 3,584 -> 2 x 20,480 28.4 (2,580); eight tokens of 4 of 60
+// experts of 2 x 1,408 x 2,048 31.5 up and 15.9 down (2,300).  The short ones are a chain of latencies
 // (launch, first copies, a few chunks, the join); the long ones are bound by the unpacking: a word of
 // eight codes is eleven instructions ahead of its mma, the ALU pipe is the busiest unit at 48 % of all
 // cycles and the issue slots at 45 %.  One pass over the codes serves up to 32 rows; tcgen05 would want
