@@ -1735,12 +1735,16 @@ def _int4_tc(what, x, rows, offsets, w, num_rows, out_dtype, row_scale=None, act
     return out
 
 
-# One matrix: the streaming kernel reads the codes once for every 32 rows (16 in 32 bits) and its
-# time goes by rows x bytes; the tensor-core kernel has some 10 to 16 us to begin and end with.
-# us, streaming / tensor cores: 2048 x 2048 64 rows 8.6 / 11.4, 128 rows 15.0 / 15.7, 192 rows 21.8 /
-# 15.9; 2048 x 6144 32 rows 13.1 / 15.8, 48 rows 22.1 / 15.9; gated 2048 x 5632 16 rows 12.1 / 16.1,
-# 32 rows 17.0 / 16.4; 32-bit 2048 x 2048 32 rows 10.7 / 14.3, 64 rows 19.4 / 16.1.
+# One matrix: the streaming kernel reads the codes once for every 32 rows (16 in 32 bits), pass after
+# pass, and its time goes by rows x bytes; the tensor-core kernel has some 6 to 13 us to begin and end
+# with.  us, streaming / tensor cores: 2048 -> 6144 32 rows 13.6 / 13.9, 64 rows 24 / 14.1; gated 2048 -> 2
+# x 5632 24 rows 16.4 / 14.5.  Small matrices leave SMs idle in every pass: 512 -> 512 64 rows 6.6 /
+# 7.5, 96 rows 9.2 / 7.5, 512 rows 42 / 8.1; 5632 -> 64 48 rows 12.8 / 10.8; 2048 -> 2048 64 rows 8.5 /
+# 11.1, 96 rows 11.9 / 12.3; 32-bit 2048 -> 2048 32 rows 10.8 / 12.3, 48 rows 15.3 / 13.1; 1024 -> 1024
+# 32 rows 6.8 / 10.6, 64 rows 12.0 / 11.8.  An eager 32-bit call on the tensor cores is three launches,
+# 24 us of the host against 10: 33 rows of 1000 -> 515 take 10.3 / 23.8 a call.
 INT4_STREAM_ROWS = 16
+INT4_STREAM_MOST_ROWS = {torch.bfloat16: 64, torch.float32: 48}
 INT4_STREAM_ROW_BYTES = {torch.bfloat16: 250e6, torch.float32: 110e6}
 # Experts (60 of 2 x 1408 x 2048 and back, us, streaming 8 / 16 rows a pass / tensor cores): 6.4 rows
 # an expert 115 / 128 / 172, 8.5 rows 136 / 129 / 172, 12.8 rows 176 / 144 / 172; 32-bit 6.4 rows
@@ -1757,7 +1761,8 @@ def _int4_product(what: str, x: torch.Tensor, w: Int4Weight, halves: int,
     if out_dtype not in (torch.float32, x.dtype):
         raise KernelError(f"{what}: results in {out_dtype} from activations in {x.dtype}")
     M = x.shape[0]
-    if M <= INT4_STREAM_ROWS or M * w._data.nbytes <= INT4_STREAM_ROW_BYTES[x.dtype]:
+    if M <= INT4_STREAM_ROWS or (M <= INT4_STREAM_MOST_ROWS[x.dtype]
+                                 and M * w._data.nbytes <= INT4_STREAM_ROW_BYTES[x.dtype]):
         if M == 0:
             return torch.empty((0, w.cols), dtype=out_dtype, device=x.device)
         return _int4_stream(what, x, None, None, w, M, out_dtype, M, activation=activation)

@@ -31,6 +31,7 @@ def kernel(request, monkeypatch):
         most = 0 if request.param == "many rows" else 1 << 62
         each = {torch.bfloat16: most, torch.float32: most}
         monkeypatch.setattr(ops(), "INT4_STREAM_ROWS", most)
+        monkeypatch.setattr(ops(), "INT4_STREAM_MOST_ROWS", each)
         monkeypatch.setattr(ops(), "INT4_STREAM_ROW_BYTES", each)
         monkeypatch.setattr(ops(), "INT4_STREAM_ROWS_PER_EXPERT", each)
     return request.param
