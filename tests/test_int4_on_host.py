@@ -192,3 +192,20 @@ def test_a_model_whose_parts_name_no_matrices_is_refused(monkeypatch):
     with pytest.raises(ValueError, match="no part of this model"):
         load_model(config_json=TINY_A, source=RandomSource(1), dtype="float32", device="cpu", ops=H,
                    int4_group=32)
+
+
+@pytest.mark.parametrize("rows,k,n,dtype,want", [
+    (1, 20480, 3584, torch.bfloat16, "few"), (16, 20480, 3584, torch.bfloat16, "few"),
+    (64, 20480, 3584, torch.bfloat16, "many"), (64, 512, 512, torch.bfloat16, "few"),
+    (65, 512, 512, torch.bfloat16, "many"), (1024, 128, 16, torch.bfloat16, "many"),
+    (48, 512, 512, torch.float32, "few"), (49, 512, 512, torch.float32, "many"),
+    (17, 20480, 3584, torch.float32, "many"), (0, 64, 64, torch.float32, "none")])
+def test_which_kernel_takes_a_call(monkeypatch, rows, k, n, dtype, want):
+    taken = []
+    monkeypatch.setattr(kernel_ops, "_int4_operands", lambda *a: None)
+    monkeypatch.setattr(kernel_ops, "_int4_stream", lambda *a, **kw: taken.append("few"))
+    monkeypatch.setattr(kernel_ops, "_int4_tc", lambda *a, **kw: taken.append("many"))
+    q = kernel_ops._int4_empty("here", (n, k), 128, 1, "meta")
+    out = kernel_ops.linear(torch.empty((rows, k), dtype=dtype, device="meta"), q)
+    assert taken == ([] if want == "none" else [want])
+    assert want != "none" or tuple(out.shape) == (0, n)
