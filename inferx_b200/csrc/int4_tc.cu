@@ -306,7 +306,7 @@ int4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
     w /= p.splits;
     const int tt = w / f_tiles;
     it.f0 = (w - tt * f_tiles) * F;
-    it.c0 = it.z * p.run;
+    it.c0 = min(p.chunks, it.z * p.run);     // (roles count chunks: c1 - c0 is never negative)
     it.c1 = min(p.chunks, it.c0 + p.run);
     if (p.offsets) {
       int lo = 0, hi = p.E;                  // the last e with tile_start[e] <= tt
@@ -791,6 +791,9 @@ static I4TPlan i4t_plan(int rows, int N, int Kp, int E, bool grouped, bool dual,
     const long long tiles = (rows < E ? rows : E) * f_tiles;
     while (rows <= 4096 && plan.splits < 16 && tiles * plan.splits * 2 <= pairs && chunks / (plan.splits * 2) >= 2)
       plan.splits *= 2;
+    // no run begins at or behind the last chunk (20 chunks in runs of 3 are seven runs, not eight)
+    const int run = (chunks + plan.splits - 1) / plan.splits;
+    plan.splits = (chunks + run - 1) / run;
     return plan;
   }
   const int most = rows > 128 && terms == 1 ? 192 : 128;
