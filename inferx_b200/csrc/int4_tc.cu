@@ -580,6 +580,10 @@ int4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
             pb[i][j] = own[i][I4_CODE_WORDS + (g + 8) * NG + j];
           }
           if (i == 1) {
+            // The next copy into this stage may not pass the reads, which no instruction has waited
+            // for yet: where the load unit is busy with results an arrival overtakes them by a
+            // microsecond, and the codes of three chunks on are what is read.
+            fence_proxy_async();
             __syncwarp();
             if (lane == 0) mbar_arrive(&empty_c[sc]);
           }
