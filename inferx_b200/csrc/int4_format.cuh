@@ -40,6 +40,7 @@ struct I4Weight {
   int E;                               // experts
   int group;
   int dual;                            // a gate and an up matrix per expert
+  int settled;                         // nothing on the device writes it any more
 };
 
 // Shared memory beyond 48 KB has to be asked for once per kernel and device.

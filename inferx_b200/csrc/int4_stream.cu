@@ -112,8 +112,7 @@ template <typename XT, bool DUAL, int NT, int GROUP, int S>
 __global__ void __launch_bounds__(I4S_THREADS, NT == 1 && sizeof(XT) == 2 ? 2 : 1)
 int4_stream_kernel(const XT* __restrict__ x, const int* __restrict__ rows,
                    const int* __restrict__ offsets, const unsigned* __restrict__ data, I4Out out,
-                   int M_single, int N, int K, int E, int strips, int chunks, int klog,
-                   int offsets_settled) {
+                   int M_single, int N, int K, int E, int strips, int chunks, int klog, int early) {
   typedef I4SCfg<XT, NT, GROUP, S> C;
   constexpr int NG = 128 / GROUP, PER = GROUP / 16;
   constexpr int TERMS = I4Frag<XT>::TERMS, ACCS = TERMS == 3 ? 2 : 1;
@@ -128,9 +127,8 @@ int4_stream_kernel(const XT* __restrict__ x, const int* __restrict__ rows,
   const int ksplit = 1 << klog, tiles = I4S_WARPS >> klog;
   const int tile = warp >> klog, ks = warp & (ksplit - 1);
   const int pos = blockIdx.x * tiles + tile;
-  // Weights are never written on the device while steps run: the first copies go out before the
-  // wait on the predecessor where the range of rows is known already.
-  const bool early = offsets == nullptr || offsets_settled != 0;
+  // The first copies of codes go out before the wait on the predecessor where the caller says that
+  // nothing on the device still writes the weights and the range of rows is known already.
   if (!early) IX_PDL_WAIT();
   int e = 0, lo = 0, hi = M_single;
   if (offsets) {
@@ -362,7 +360,7 @@ struct I4SCall {
   const int *rows, *offsets;
   const void* data;
   I4Out out;
-  int M, N, K, E, active, settled;
+  int M, N, K, E, active, early;
 };
 
 template <typename XT, bool DUAL, int NT, int GROUP, int S>
@@ -386,7 +384,7 @@ static int i4s_launch2(const I4SCall& c, cudaStream_t stream) {
   if (e != cudaSuccess) return (int)e;
   ix_launch(kern, dim3((sets + tiles - 1) / tiles, c.active), dim3(I4S_THREADS), C::SMEM, stream,
             (const XT*)c.x, c.rows, c.offsets, (const unsigned*)c.data, c.out, c.offsets ? 0 : c.M,
-            c.N, c.K, c.E, strips, chunks, klog, c.settled);
+            c.N, c.K, c.E, strips, chunks, klog, c.early);
   return ix_launch_status();
 }
 
@@ -403,7 +401,8 @@ static int i4s_launch(const I4SCall& c, cudaStream_t stream) {
 // x: [*, K] fp32 or bf16, K a multiple of 8 that ends in the weight's last chunk, 16-byte aligned;
 // out: [rows, N] fp32 (wide) or bf16.  offsets == null: one matrix with M rows.  active: the most
 // groups that can have rows (0: all).  offsets_settled: nonzero when `offsets` was written at least two
-// launches back in the stream.
+// launches back in the stream.  w->settled: the same of the weights, for good; where it is 0 (they have
+// just been quantised or packed, perhaps by the launch before) they are read behind the wait.
 IX_API int ix_int4_stream(const I4Weight* w, const void* x, int x_dtype, const int* rows,
                           const int* offsets, void* out, int wide, int M, int K, int rows_per_pass,
                           int active, int offsets_settled, const float* row_scale, int plain,
@@ -417,7 +416,7 @@ IX_API int ix_int4_stream(const I4Weight* w, const void* x, int x_dtype, const i
   if (((uintptr_t)x | (uintptr_t)w->data) & 15) return IX_ERR_ALIGN;
   if (active <= 0 || active > E) active = E;
   const I4SCall c = {x, rows, offsets, w->data, {out, wide, row_scale, plain}, M, w->N, K, E, active,
-                     offsets_settled};
+                     w->settled != 0 && (!offsets || offsets_settled != 0)};
   const int nt = rows_per_pass > 16 ? 4 : rows_per_pass > 8 ? 2 : 1;
 #define I4S_GO(T, D, NT, G) return i4s_launch<T, D, NT, G>(c, stream)
 // (32 rows of three terms each would not fit the registers: fp32 takes 16 a pass)

@@ -1513,7 +1513,7 @@ INT4_LAYOUT_ROWS, INT4_LAYOUT_K = 16, 128     # a strip of rows, a chunk of k
 class _Int4Record(ctypes.Structure):
     """What the products' entry points want to know of a weight (csrc/int4_format.cuh)."""
     _fields_ = [("data", ctypes.c_void_p), ("cols", ctypes.c_int), ("experts", ctypes.c_int),
-                ("group", ctypes.c_int), ("dual", ctypes.c_int)]
+                ("group", ctypes.c_int), ("dual", ctypes.c_int), ("settled", ctypes.c_int)]
 
 
 class Int4Weight:
@@ -1536,7 +1536,8 @@ class Int4Weight:
         self.cols, self.inner = self.shape[-2] // halves, self.shape[-1]
         self.device_index = data.get_device()
         # what a product's entry point reads, and where (made once: threads share a weight)
-        self._record = _Int4Record(data.data_ptr(), self.cols, self.experts, group_size, halves - 1)
+        self._record = _Int4Record(data.data_ptr(), self.cols, self.experts, group_size,
+                                   halves - 1, 0)
         self.at = ctypes.addressof(self._record)
 
     def __reduce__(self):
@@ -1545,6 +1546,20 @@ class Int4Weight:
     @property
     def data(self) -> torch.Tensor:
         return self._data
+
+    def settle(self) -> "Int4Weight":
+        """Waits for the device, and says that nothing on it writes this weight from now on: where
+        launches overlap (``set_dependent_launch``), products may then fetch its codes while the
+        kernel before them still runs.  A weight that has just been made is not settled, nor is a
+        copy of one that is."""
+        if self._data.is_cuda:
+            torch.cuda.synchronize(self._data.device)
+        self._record.settled = 1
+        return self
+
+    @property
+    def settled(self) -> bool:
+        return bool(self._record.settled)
 
     @property
     def device(self):

@@ -56,7 +56,10 @@ def hold_in_int4(part, ctx: BuildContext) -> int:
     for name, halves in getattr(part, "int4_weights", {}).items():
         w = getattr(part, name)
         if isinstance(w, torch.Tensor):
-            setattr(part, name, ctx.ops.quantize_int4(w.contiguous(), ctx.int4_group, halves))
+            held_w = ctx.ops.quantize_int4(w.contiguous(), ctx.int4_group, halves)
+            if hasattr(held_w, "settle"):      # (steps only read it)
+                held_w.settle()
+            setattr(part, name, held_w)
             held += 1
     for name in getattr(part, "int4_parts", ()):
         held += hold_in_int4(getattr(part, name), ctx)
