@@ -14,14 +14,19 @@
 // mma.m16n8k16 (k in an order that the activations' 8-byte loads follow too), and, as four registers of
 // pairs, sixteen rows by sixteen k of an operand in tensor memory (the 16x256b shape).
 //
-// Parameters.  [row 0..15][group of the chunk]: one word, the scale in the low half, 128 + zero as
-// bfloat16 in the high half.  (The zero point as a nibble would be 1.5 of 67 bytes a group less; the
-// word needs no arithmetic before its use.)
+// Parameters.  [row 0..15][group of the chunk]: one word, the scale times 2^11 in the low half, 2^-4 +
+// zero * 2^-11 as bfloat16 in the high half.  (The zero point as a nibble would be 1.5 of 67 bytes a
+// group less; the word needs no arithmetic before its use.)
 //
-// A code c becomes the bfloat16 128 + c by setting its bits below 0x4300, and 128 + c - (128 + zero)
-// is exact: products of activations with codes are formed from whole numbers of -15..15, summed in
-// fp32 over a group, and the group's scale multiplies the sum in fp32.  Padding codes equal their
-// group's zero point, padding rows and groups have scale 0.
+// A code c becomes the bfloat16 2^-4 + c * 2^-11 by setting its bits below 0x3d80, and the difference
+// to 2^-4 + zero * 2^-11 is exact: products of activations with codes are formed from multiples of
+// 2^-11 up to 15 * 2^-11, summed in fp32 over a group, and the group's scale multiplies the sum in
+// fp32.  128 of them are less than one, so the sum of a group does not overflow where the activations
+// have not (as whole numbers up to 15 they did from 1.7e35 on), and down to activations of 2^-133, the
+// last bit that bfloat16 has, their products are numbers that fp32 holds.  A scale that 2^11 would
+// take out of bfloat16's range is held as it is, over codes as whole numbers: 128 + zero (0x4300 +
+// zero) in the high half says so.
+// Padding codes equal their group's zero point, padding rows and groups have scale 0.
 #pragma once
 #include "common.cuh"
 
@@ -62,13 +67,33 @@ __host__ __device__ static inline long long i4_chunks(long long k) {
   return (k + I4_CHUNK_K - 1) / I4_CHUNK_K;
 }
 
+#define I4_UNIT 0x3d80u                // 2^-4, whose last bit is 2^-11
+#define I4_WHOLE 0x4300u               // 128, whose last bit is 1
+
+// scale (bfloat16) and zero point as a parameter, and back
+__device__ __forceinline__ unsigned i4_param(__nv_bfloat16 scale, int zero) {
+  const float s = __bfloat162float(scale);
+  // (2^11 is exact: a smaller scale only leaves the subnormal numbers)
+  if (fabsf(s) < 0x1p116f)
+    return (unsigned)__bfloat16_as_ushort(__float2bfloat16_rn(s * 2048.f)) |
+           ((I4_UNIT + (unsigned)zero) << 16);
+  return (unsigned)__bfloat16_as_ushort(scale) | ((I4_WHOLE + (unsigned)zero) << 16);
+}
+__device__ __forceinline__ int i4_param_zero(unsigned param) { return (param >> 16) & 15; }
+__device__ __forceinline__ unsigned short i4_param_scale(unsigned param) {
+  const float s = __uint_as_float(param << 16);
+  return (param >> 20) == (I4_UNIT >> 4)
+             ? __bfloat16_as_ushort(__float2bfloat16_rn(s * (1.f / 2048.f)))
+             : (unsigned short)param;
+}
+
 __device__ __forceinline__ float i4_scale(unsigned param) { return __uint_as_float(param << 16); }
-// 128 + zero in both halves
+// the zero point's number in both halves
 __device__ __forceinline__ unsigned i4_sub(unsigned param) { return __byte_perm(param, 0, 0x3232); }
 
 // Nibbles i and i + 4 of a word, less the zero point: two neighbouring k.
 __device__ __forceinline__ unsigned i4_pair(unsigned word, int i, unsigned sub) {
-  unsigned q = ((word >> (4 * i)) & 0x000f000fu) | 0x43004300u;
+  unsigned q = ((word >> (4 * i)) & 0x000f000fu) | (sub & 0xfff0fff0u);
   const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&q),
                                    *reinterpret_cast<const __nv_bfloat162*>(&sub));
   return *reinterpret_cast<const unsigned*>(&d);

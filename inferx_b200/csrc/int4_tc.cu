@@ -20,7 +20,7 @@
 //   4-11   take each finished group's sums out of tensor memory, a weight row a lane, add scale * sum to
 //          fp32 registers, and leave an item's results in shared memory;
 //   12-19  unpack, four the even chunks and four the odd ones, two strips a warp: a lane's sixteen bytes
-//          of codes, less their zero points, are whole numbers that lie in registers as tensor memory
+//          of codes, less their zero points, are numbers of five bits that lie in registers as tensor memory
 //          wants them (16 rows by 256 bits);
 //   20-23  finish and store the results of an item while the next one is under way.
 // Rows of a DUAL item lie as 16 gate rows, the 16 up rows of the same columns, and so on.

@@ -43,10 +43,6 @@ __device__ __forceinline__ bf16 i4_group_scale(float lo, float hi) {
   return __float2bfloat16_rn(t);
 }
 
-__device__ __forceinline__ unsigned i4_param(bf16 scale, int zero) {
-  return (unsigned)__bfloat16_as_ushort(scale) | (0x43000000u + ((unsigned)zero << 16));
-}
-
 // Where a warp works: matrix, strip, chunk; false behind the last.
 struct I4Place {
   long long m;
@@ -314,8 +310,8 @@ i4_unpack_kernel(const unsigned* __restrict__ data, unsigned char* __restrict__ 
       const int group = p.chunk * NG + n;
       if (group >= groups) continue;
       const unsigned param = data[block + I4_CODE_WORDS + (g + side * 8) * NG + n];
-      scales[r * groups + group] = __ushort_as_bfloat16((unsigned short)param);
-      zeros[r * groups + group] = (unsigned char)((param >> 16) - 0x4300u);
+      scales[r * groups + group] = __ushort_as_bfloat16(i4_param_scale(param));
+      zeros[r * groups + group] = (unsigned char)i4_param_zero(param);
     }
   }
 }
