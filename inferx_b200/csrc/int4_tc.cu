@@ -15,7 +15,8 @@
 // warps, a chunk of 128 k at a time:
 //   0      brings the rows into a ring of stages (TMA, 128-byte swizzle);
 //   1      the first block's issues the MMAs for both, a group of k into one of two accumulators in
-//          tensor memory; the second block's tells the first that its own operands are there;
+//          tensor memory; the second block's tells the first that its weights are there and its sums
+//          taken (its rows' copies report to the first block's barrier themselves);
 //   2      brings the codes and parameters of the block's eight strips (one bulk copy, DUAL two);
 //   4-11   take each finished group's sums out of tensor memory, a weight row a lane, add scale * sum to
 //          fp32 registers, and leave an item's results in shared memory;
@@ -109,31 +110,36 @@ __device__ __forceinline__ void i4t_copy(void* to, const void* from, unsigned by
       "l"(from), "r"(bytes), "r"(smem_u32(bar))
       : "memory");
 }
-// Arrives at a barrier of the other block.  Of the block's own scope, as the waits behind it are: what
-// it announces is read by MMAs, by the asynchronous proxy that the operands' writers have fenced theirs
-// into, and not by loads of a thread.  (Released at cluster scope an arrival takes some 1,400 cycles,
-// more than a chunk's MMAs.)
-__device__ __forceinline__ void i4t_arrive_at(unsigned bar) {
-  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-// Bounded wait; its polls sleep in the barrier unit, up to I4T_NAP ns each.
+// Bounded wait; its polls sleep in the barrier unit, up to I4T_NAP ns each.  PAIR: for a barrier that
+// the other block and its copies arrive at too.
+template <bool PAIR>
 __device__ __forceinline__ bool i4t_try(unsigned long long* bar, unsigned parity) {
   unsigned ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity), "r"(I4T_NAP)
-      : "memory");
+  if (PAIR)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity), "r"(I4T_NAP)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity), "r"(I4T_NAP)
+        : "memory");
   return ok != 0;
 }
+template <bool PAIR = false>
 __device__ __forceinline__ bool i4t_wait(unsigned long long* bar, unsigned parity,
                                          volatile int* abort_flag) {
-  if (i4t_try(bar, parity)) return true;
+  if (i4t_try<PAIR>(bar, parity)) return true;
   const long long begin = clock64();
   while (clock64() - begin < I4T_WAIT_CLOCKS) {
-    if (i4t_try(bar, parity)) return true;
+    if (i4t_try<PAIR>(bar, parity)) return true;
     if (*abort_flag) return false;
   }
   return false;
@@ -234,10 +240,15 @@ int4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
   float* stage = reinterpret_cast<float*>(xs + C::X_RING * C::X_STAGE);   // [row of the tile][128]
   unsigned char* cs = reinterpret_cast<unsigned char*>(stage + BT * 128);
   unsigned short* scales = reinterpret_cast<unsigned short*>(cs + C::C_RING * 8 * C::C_BYTES);
-  // A group may be multiplied: on a chunk's first group the block's operands are there (four unpacking
-  // warps and the rows' bytes), an accumulator's sums are taken (eight warps), and, in the first block,
-  // the second one is as far.  One barrier for all of it, as a wait costs the issuing warp hundreds of
-  // cycles even where nothing is waited for.
+  // A group may be multiplied: on a chunk's first group the block's weights are there (four unpacking
+  // warps), an accumulator's sums are taken (eight warps), and, in the first block, the second one is as
+  // far and both blocks' rows are there.  One barrier for all of it, as a wait costs the issuing warp
+  // hundreds of cycles even where nothing is waited for.
+  // The second block's arrival is relaxed: its threads' weights and sums are tensor memory, which the
+  // tcgen05 fences on both sides order.  Its rows lie in shared memory, and their copies report
+  // to the first block's barrier themselves, which releases them to the cluster.  (An arrival that
+  // releases what threads have written takes some 1,400 cycles, more than a chunk's MMAs; 2,048 rows,
+  // 2,048 -> 6,144 with the rows announced that way from a warp of their own 61.8 us, as it is 57.4.)
   __shared__ __align__(8) unsigned long long go[I4T_DONE][NG];
   // Codes of a chunk are there.  Two barriers for every stage, chunks in turn, so that a barrier's
   // chunks are all unpacked by the same four warps: a wait for a phase is only right where the phase
@@ -278,7 +289,8 @@ int4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
   }
   if (threadIdx.x == 0) {
     for (int s = 0; s < I4T_DONE; ++s)
-      for (int q = 0; q < NG; ++q) mbar_init(&go[s][q], (q == 0 ? 13 : 8) + (rank == 0 ? 1 : 0));
+      for (int q = 0; q < NG; ++q)
+        mbar_init(&go[s][q], q == 0 ? (rank == 0 ? 14 : 12) : (rank == 0 ? 9 : 8));
     for (int s = 0; s < 2 * C::C_RING; ++s) mbar_init(&full_c[s], 1);
     for (int s = 0; s < C::C_RING; ++s) mbar_init(&empty_c[s], 4);
     for (int s = 0; s < I4T_DONE; ++s) mbar_init(&done[s], 1);
@@ -342,6 +354,7 @@ int4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");
     if (warp == 0) {
+      const unsigned first_block = tc_of_rank(&go[0][0], 0);
       int n = 0;                             // chunks so far, over all items
       bool ok = true;
       for (int w = first; w < n_items && ok; w += step) {
@@ -349,7 +362,7 @@ int4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
         if (it.n <= 0) continue;
         const int half = ((it.n + 31) & ~31) / 2;              // rows of this block
         const int boxes = (half + C::BOX - 1) / C::BOX;
-        // a lane a box: term, 64 k, 32 rows
+        // a lane a box: term, 64 k, a quarter of the tile's rows
         const int box = lane % boxes, sub = lane / boxes & 1, term = lane / (2 * boxes);
         for (int c = it.c0; c < it.c1; ++c, ++n) {
           const int s = n % C::X_RING;
@@ -358,24 +371,28 @@ int4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
             ok = wait(&done[before % I4T_DONE], before / I4T_DONE & 1);
             if (!ok) break;
           }
-          if (lane == 0)
-            mbar_expect_tx(&go[n % I4T_DONE][0], (unsigned)(TERMS * 2 * boxes * C::BOX * 64 * 2));
+          // both blocks' bytes (the second's may land before they are expected: the phase is not over
+          // without this arrival, and its copies are not sent before the last phase is)
+          if (rank == 0 && lane == 0)
+            mbar_expect_tx(&go[n % I4T_DONE][0],
+                           (unsigned)(2 * TERMS * 2 * boxes * C::BOX * 64 * 2));
           __syncwarp();
           if (term < TERMS)
-            tma_load_2d(xs + s * C::X_STAGE + (term * 2 + sub) * C::X_TILE +
-                            box * (C::BOX * 64 * 2),
-                        &map_x, c * 128 + sub * 64,
-                        term * p.plane_rows + it.m0 + rank * half + box * C::BOX,
-                        &go[n % I4T_DONE][0]);
+            tc_load_pair(xs + s * C::X_STAGE + (term * 2 + sub) * C::X_TILE +
+                             box * (C::BOX * 64 * 2),
+                         &map_x, c * 128 + sub * 64,
+                         term * p.plane_rows + it.m0 + rank * half + box * C::BOX,
+                         first_block + (n % I4T_DONE) * NG * 8);
           __syncwarp();
         }
       }
       if (lane == 0) {
         if (!ok && !*abortp) { atomicExch(p.status, I4T_ERR_COPY); *abortp = 1; }
         // copies in flight land before the block's shared memory goes away, whatever the others do
+        // (a wait that nothing ends takes its full limit, thousands of times as long as a copy)
         if (!ok)
           for (int f = max(0, n - C::X_RING); f < n; ++f)
-            mbar_drain(&go[f % I4T_DONE][0], f / I4T_DONE & 1);
+            mbar_drain(&done[f % I4T_DONE], f / I4T_DONE & 1);
         else if (n > 0)
           mbar_drain(&done[(n - 1) % I4T_DONE], (n - 1) / I4T_DONE & 1);
       }
@@ -394,12 +411,15 @@ int4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
           const unsigned ad = tmem_base + 2 * BT + (n % C::A_RING) * 64;
           const unsigned long long xd = umma_desc(xs + (n % C::X_RING) * C::X_STAGE);
           for (int q = 0; q < NG; ++q, ++group) {
-            ok = wait(&go[slot][q], n / I4T_DONE & 1);
+            // (one wait for both blocks: with a wait in either branch a chunk takes 3 % longer, and
+            // with groups of 64 17 %)
+            ok = __all_sync(0xffffffffu,
+                            i4t_wait<true>(&go[slot][q], n / I4T_DONE & 1, abortp));
             if (!ok) break;
             tc_fence_after();
             if (rank != 0) {
               tc_fence_before();
-              if (i4t_elect()) i4t_arrive_at(first_block + (slot * NG + q) * 8);
+              if (i4t_elect()) tc_arrive_relaxed_at(first_block + (slot * NG + q) * 8);
               __syncwarp();
               continue;
             }
