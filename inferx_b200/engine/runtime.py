@@ -68,6 +68,10 @@ def load_model(model_dir: Optional[str] = None, *, dtype="bfloat16", device="cud
     model.load(src, where)
     if isinstance(src, CheckpointSource) and source is None:
         src.close()
+    if int4_group and dev.type == "cuda":
+        # the matrices that codes have replaced go back to the device, where the cache is sized from
+        # what is free
+        torch.cuda.empty_cache()
     return cfg, model
 
 
