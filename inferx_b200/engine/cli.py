@@ -56,7 +56,8 @@ def build_parser() -> argparse.ArgumentParser:
     ap.add_argument("--tensor-parallel-size", type=int, default=1)
     ap.add_argument("--device", default="cuda")
     ap.add_argument("--quantization", "-q", default=None,
-                    help="int4: projections, feed-forwards and experts are held in four bits")
+                    help="int4: attention's projections, feed-forwards and experts are held in "
+                    "four bits; mixers of other kinds keep their matrices")
     ap.add_argument("--quantization-group", type=int, default=128, choices=[32, 64, 128],
                     help="entries of a matrix's row that share a scale and a zero point")
     ap.add_argument("--kv-cache-dtype", default="auto")
@@ -180,6 +181,9 @@ def main(argv=None) -> int:
         quantization=args.quantization, quantization_group=args.quantization_group))
     log("info", f"model ready in {time.time() - t0:.1f}s",
         cache_pages=engine.stats()["pages_total"], page_tokens=args.block_size)
+    if "int4_share" in engine.stats():
+        log("info", "weights in four bits, the layers' other matrices as they were",
+            share=engine.stats()["int4_share"])
     if args.v > 0:
         log("debug", "engine", config=json.dumps(engine.model_config.to_json(), sort_keys=True)
             if hasattr(engine.model_config, "to_json") else str(engine.model_config))

@@ -266,7 +266,9 @@ class Engine:
 
     def stats(self) -> Dict[str, Any]:
         mgr = self.runtime.manager
+        held = self.runtime.model.int4_share if self.config.int4_group() else None
         return {
+            **({} if held is None else {"int4_share": round(held, 4)}),
             "steps": self.scheduler.steps,
             "preemptions": self.scheduler.preemptions,
             "tokens_generated": self.tokens_generated,

@@ -45,8 +45,9 @@ def load_model(model_dir: Optional[str] = None, *, dtype="bfloat16", device="cud
                config_json: Optional[Mapping[str, Any]] = None,
                source: Optional[WeightSource] = None, ops=None, int4_group: int = 0):
     """(typed config, DecoderModel with weights bound).  ``int4_group`` > 0: the matrices that
-    the parts name (projections of attention, feed-forwards, experts) are held in four bits
-    with a scale for so many entries; embedding, head, router, norms and biases are not.
+    the parts name (projections of attention over keys and values, feed-forwards, experts) are
+    held in four bits with a scale for so many entries; embedding, head, router, norms, biases
+    and the matrices of other mixers are not (``model.int4_share``: the share that is).
 
     Either ``model_dir`` (config.json + safetensors) or ``config_json`` with a
     ``source`` (for instance a ``RandomSource`` on the device)."""

@@ -68,6 +68,15 @@ def hold_in_int4(part, ctx: BuildContext) -> int:
     return held
 
 
+def int4_entries(part) -> int:
+    """How many entries of a part's matrices are held in four bits."""
+    if part is None:
+        return 0
+    held = (getattr(part, name) for name in getattr(part, "int4_weights", {}))
+    return sum(w.numel() for w in held if w is not None and not isinstance(w, torch.Tensor)) \
+        + sum(int4_entries(getattr(part, name)) for name in getattr(part, "int4_parts", ()))
+
+
 @dataclass(frozen=True)
 class PagedKvNeed:
     """A record per token, kept in pages.  ``entries`` names the tensors of the record:

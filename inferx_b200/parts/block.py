@@ -18,7 +18,8 @@ import torch
 
 from ..weights import loader as wl
 from ..weights.loader import TensorDecl
-from .base import BuildContext, LayerCache, PendingSum, StepContext, hold_in_int4
+from .base import (BuildContext, LayerCache, PendingSum, StepContext, hold_in_int4,
+                   int4_entries)
 from .registry import build_part, register_part
 from .streams import read_streams
 
@@ -251,11 +252,19 @@ class DecoderModel:
         self.stream_tables = {n: t for n, t in own.items()
                               if n not in (self.spec.embed_name, self.spec.head_name)}
         # (the matrices of stream projections live in the same table, by name)
-        matrices = 0
+        matrices = held_entries = entries = 0
         for b in self.blocks:
             for part in b.parts():
-                part.bind(fetch(part.tensors()))
+                decls = part.tensors()
+                tensors = fetch(decls)
+                entries += sum(t.numel() for t in (tensors.get(d.name) for d in decls
+                                                   if d.keep == "param")
+                               if t is not None and t.dim() >= 2 and min(t.shape) > 1)
+                part.bind(tensors)
                 matrices += hold_in_int4(part, self.ctx)
+                held_entries += int4_entries(part)
+        # how much of the layers' matrices is held in four bits (parts that name none keep theirs)
+        self.int4_share = min(1.0, held_entries / max(1, entries))
         if self.ctx.int4_group and not matrices:
             raise ValueError("no part of this model names matrices that can be held in four bits")
         self.final_norm.bind(fetch(self.final_norm.tensors()))
