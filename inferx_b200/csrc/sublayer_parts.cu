@@ -292,8 +292,8 @@ __device__ __forceinline__ float clamped_glu(float g, float u, float limit, floa
   return g / (1.0f + expf(-alpha * g)) * (u + up_shift);
 }
 
-template <typename TA>
-__global__ void glu_clamped_kernel(const TA* __restrict__ gu, TA* __restrict__ out, long long total,
+template <typename TA, typename TO>
+__global__ void glu_clamped_kernel(const TA* __restrict__ gu, TO* __restrict__ out, long long total,
                                    int I, float limit, float alpha, float up_shift) {
   IX_PDL_WAIT();
   for (long long idx = (long long)blockIdx.x * blockDim.x + threadIdx.x; idx < total;
@@ -302,7 +302,7 @@ __global__ void glu_clamped_kernel(const TA* __restrict__ gu, TA* __restrict__ o
     const int j = (int)(idx - t * I);
     const float g = to_f32(gu[t * 2 * I + j]);
     const float u = to_f32(gu[t * 2 * I + I + j]);
-    out[idx] = from_f32<TA>(clamped_glu(g, u, limit, alpha, up_shift));
+    out[idx] = from_f32<TO>(clamped_glu(g, u, limit, alpha, up_shift));
   }
 }
 
@@ -344,10 +344,12 @@ glu_clamped_bf16_vec_kernel(const uint4* __restrict__ gu, uint4* __restrict__ ou
   }
 }
 
-IX_API int ix_glu_clamped(const void* gu, void* out, int act_dtype, int T, int I, float limit,
-                          float alpha, float up_shift, cudaStream_t stream) {
+// gu and out have one element type, or gu is fp32 and out bfloat16.
+IX_API int ix_glu_clamped(const void* gu, int act_dtype, void* out, int out_dtype, int T, int I,
+                          float limit, float alpha, float up_shift, cudaStream_t stream) {
   if (T <= 0) return IX_OK;
   if (I <= 0) return IX_ERR_SIZE;
+  if (act_dtype == IX_BF16 && out_dtype != IX_BF16) return IX_ERR_DTYPE;
   const long long total = (long long)T * I;
   if (act_dtype == IX_BF16 && I % 8 == 0 && (((uintptr_t)gu | (uintptr_t)out) & 15) == 0 &&
       total / 8 < (1LL << 30)) {
@@ -360,9 +362,15 @@ IX_API int ix_glu_clamped(const void* gu, void* out, int act_dtype, int T, int I
   }
   long long blocks = (total + 255) / 256;
   if (blocks > 148 * 16) blocks = 148 * 16;
-  IX_DISPATCH_DTYPE(act_dtype, TA,
-                    ix_launch(glu_clamped_kernel<TA>, dim3((int)blocks), dim3(256), 0, stream,
-                              (const TA*)gu, (TA*)out, total, I, limit, alpha, up_shift));
+  if (act_dtype == IX_BF16) {
+    ix_launch(glu_clamped_kernel<bf16, bf16>, dim3((int)blocks), dim3(256), 0, stream,
+              (const bf16*)gu, (bf16*)out, total, I, limit, alpha, up_shift);
+    return ix_launch_status();
+  }
+  if (act_dtype != IX_F32) return IX_ERR_DTYPE;
+  IX_DISPATCH_DTYPE(out_dtype, TO,
+                    ix_launch(glu_clamped_kernel<float, TO>, dim3((int)blocks), dim3(256), 0, stream,
+                              (const float*)gu, (TO*)out, total, I, limit, alpha, up_shift));
   return ix_launch_status();
 }
 

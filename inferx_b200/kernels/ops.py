@@ -449,6 +449,8 @@ def qkv_project_applies(x: torch.Tensor, w: torch.Tensor, heads: int, kv_heads: 
     """Whether ``qkv_project_rope_append`` takes this step: bfloat16, a few tokens, a full
     rotation or none."""
     if isinstance(w, Int4Weight):
+        # (q, k and v are then rounded to the run's type between the product and the rotation, as
+        # in steps of many tokens; that kernel alone keeps them in fp32)
         return False
     return bool(USE_FUSED_QKV and x.is_cuda and x.dtype == torch.bfloat16
                 and w.dtype == torch.bfloat16 and x.is_contiguous()
@@ -1870,14 +1872,20 @@ def group_norm_rows(resid: torch.Tensor, rows: Optional[torch.Tensor], gain: tor
     return out
 
 
-def glu_clamped(gu: torch.Tensor, limit: float, alpha: float, up_shift: float):
-    """[T, 2I] (gate | up) -> min(g, L) * sigmoid(alpha * min(g, L)) * (clamp(u, -L, L) + up_shift)."""
+def glu_clamped(gu: torch.Tensor, limit: float, alpha: float, up_shift: float,
+                out_dtype: Optional[torch.dtype] = None):
+    """[T, 2I] (gate | up) -> min(g, L) * sigmoid(alpha * min(g, L)) * (clamp(u, -L, L) + up_shift),
+    in ``gu``'s type, or in bfloat16 from float32."""
     _chk("gu", gu)
+    out_dtype = out_dtype or gu.dtype
+    if out_dtype not in (gu.dtype, torch.bfloat16):
+        raise KernelError(f"glu_clamped: {out_dtype} from {gu.dtype}")
     T, two_i = gu.shape
     if two_i % 2:
         raise KernelError("glu_clamped: width must be even (gate | up)")
-    out = torch.empty((T, two_i // 2), dtype=gu.dtype, device=gu.device)
-    _check(_lib().ix_glu_clamped(_ptr(gu), _ptr(out), _dtype_code(gu), T, two_i // 2,
+    out = torch.empty((T, two_i // 2), dtype=out_dtype, device=gu.device)
+    _check(_lib().ix_glu_clamped(_ptr(gu), _dtype_code(gu), _ptr(out), _dtype_code(out), T,
+                                 two_i // 2,
                                  ctypes.c_float(limit), ctypes.c_float(alpha),
                                  ctypes.c_float(up_shift), _stream()), "glu_clamped")
     _count()
@@ -1889,7 +1897,11 @@ def gate_up_glu_clamped(x: torch.Tensor, w_gate_up: torch.Tensor, limit: float, 
     """Front half of a clamped-GLU feed-forward: the fused gate|up product and the
     activation; one weight-streaming kernel for a few rows."""
     if isinstance(w_gate_up, Int4Weight):
-        return glu_clamped(linear(x, w_gate_up), limit, alpha, up_shift)
+        # a few rows: gate and up stay in fp32 up to the activation, as in the kernel below; with
+        # many rows they pass through memory in the run's type, as there
+        few = torch.float32 if x.shape[0] <= SMALL_M_DENSE_ROWS else None
+        return glu_clamped(linear(x, w_gate_up, out_dtype=few), limit, alpha, up_shift,
+                           out_dtype=x.dtype)
     _chk("x", x)
     _chk("w_gate_up", w_gate_up, x.dtype)
     M = x.shape[0]
