@@ -1592,6 +1592,10 @@ def _int4_empty(what: str, shape, group_size: int, halves: int, device) -> Int4W
     chunks = -(-shape[-1] // INT4_LAYOUT_K)
     data = torch.empty((matrices, chunks, strips, 256 + 16 * (128 // group_size)),
                        dtype=torch.int32, device=device)
+    if data.is_cuda and not torch.cuda.is_current_stream_capturing():
+        # the word that a product's waits report to: made now, since a product that is the first to
+        # want it may be recorded, and the word would then be cleared by the replays alone
+        _tc_status(data.device)
     return Int4Weight(shape, halves, group_size, data)
 
 
