@@ -18,15 +18,18 @@
 // ones summed apart from the first.  The warps of a block split K by chunks and join their sums through
 // shared memory in warp order, so a row's result does not depend on which rows share its tile.
 //
-// Measured (bfloat16, groups of 128; us, GB/s of codes): one row, 2,048 -> 2,048 2.9 (725); eight rows,
-// 5,632 -> 2,048 5.0 (1,140); eight rows gated, 3,584 -> 2 x 20,480 28.4 (2,580); eight tokens of 4 of 60
-// experts of 2 x 1,408 x 2,048 31.5 up and 15.9 down (2,300).  The short ones are a chain of latencies
-// (launch, first copies, a few chunks, the join); the long ones are bound by the unpacking: a word of
-// eight codes is eleven instructions ahead of its mma, the ALU pipe is the busiest unit at 48 % of all
-// cycles and the issue slots at 45 %.  One pass over the codes serves up to 32 rows; tcgen05 would want
-// 128 weight rows by 128 k unpacked into tensor memory before its first product, which is the other
-// kernel's business.  Blocks that stay and take one piece of work after the other were built and are slower, and so
-// were shifts by multiplication.
+// Measured (bfloat16, groups of 128, weights from DRAM; us, GB/s of codes): one row, 2,048 -> 2,048 3.5
+// (600), gated 2,048 -> 2 x 5,632 7.6 (1,520); eight rows, 5,632 -> 2,048 5.3 (1,100), gated 3,584 -> 2 x
+// 20,480 25.0 (2,930); eight tokens of 4 of 60 experts of 2 x 1,408 x 2,048 27.1 up and 14.9 down (2,900
+// and 2,600).  What bounds it is latency: the short calls are one chain (launch, first copies, a few chunks,
+// the join: 19 % of issue slots used, memory 16 % busy), and in the long ones nothing is busy either
+// (issue slots 44 %, ALU pipe 41 %, memory 37 %).  Registers (120 a thread) and rings let two blocks onto
+// an SM, 14.7 warps in the mean, and a warp is ready every sixth cycle: its time goes in about equal
+// parts to the ring's loads, results of fixed latency, the ALU's turns and the other warps'.  In 32 bits
+// three terms and their sums leave one block an SM: eight tokens of the experts 57 us up, 29 down.  One
+// pass over the codes serves up to 32 rows; tcgen05 would want 128 weight rows by 128 k unpacked into
+// tensor memory before its first product, which is the other kernel's business.  Blocks that stay and
+// take one piece of work after the other were built and are slower, and so were shifts by multiplication.
 #include "int4_format.cuh"
 
 #define I4S_THREADS 256
@@ -369,9 +372,9 @@ static int i4s_launch2(const I4SCall& c, cudaStream_t stream) {
   const int strips = (int)i4_strips(c.N), chunks = (int)i4_chunks(c.K);
   const int sets = DUAL ? strips : (strips + S - 1) / S;
   // K is split over the warps of a block until there are 32 warps for every SM, as long as a warp
-  // keeps four chunks (us at 8 rows, 1 / 2 / 4 / 8 warps: gated 3584 x 20480 42 / 33 / 28 / 30; 25
-  // experts of 2 x 1408 x 2048 34 / 32 / 34 / 42); where that leaves SMs idle it is split further (2048
-  // x 6144 9 / 6.5 / 6.2 / 6.5, 2048 x 2048 8.6 / 5.9 / 4.2 / 3.6).
+  // keeps four chunks (us at 8 rows, 1 / 2 / 4 / 8 warps: gated 3584 x 20480 36 / 29 / 26 / 27; 27
+  // experts of 2 x 1408 x 2048 29 / 27 / 29 / 34); where that leaves SMs idle it is split further (2048
+  // x 6144 9.1 / 6.5 / 6.2 / 6.5, 2048 x 2048 8.8 / 6.0 / 4.3 / 3.6).
   int klog = 0;
   const long long warps = (long long)sets * c.active;
   while (klog < 3 && (1 << klog) < chunks && (warps << klog) < 148 * 32 &&

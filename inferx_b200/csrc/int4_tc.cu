@@ -29,13 +29,14 @@
 // a group are the tensor cores' fp32, and a group's scale multiplies in fp32: no weight is rounded to
 // bfloat16.
 //
-// Measured (bfloat16, groups of 128): 2,048 rows, 2,048 -> 6,144 57.5 us (897 TFLOP/s); 4,096 rows, 3,584 ->
-// 4,096 111 us (1,085; a bfloat16 library product alone reaches 1,670); gated, 2,048 rows, 2,048 -> 2 x
-// 5,632 96 us (989); 60 experts of 2 x 1,408 x 2,048 with 137 rows each 133 us (710).  What bounds it: a chunk
+// Measured (bfloat16, groups of 128): 2,048 rows, 2,048 -> 6,144 57.7 us (893 TFLOP/s); 4,096 rows, 3,584 ->
+// 4,096 111 us (1,081; a bfloat16 library product alone reaches 1,670); gated, 2,048 rows, 2,048 -> 2 x
+// 5,632 97 us (976); 60 experts of 2 x 1,408 x 2,048 with 137 rows each 132 us (715).  What bounds it: a chunk
 // of 192 rows takes 1,330 cycles where its MMAs are 768.  The summing warps need 700 for their 96 columns
 // and 630 more from one accumulator to the next (the arrival, two waits), and an operand stage is full
 // again 1,300 after its MMAs have run; tensor memory has room for two accumulators and two stages.
-// Groups of 64 or 32 have two or four sums a chunk to take: 2,048 -> 6,144 with groups of 64 80.6 us.
+// Groups of 64 or 32 have two or four sums a chunk to take: 2,048 -> 6,144 80.6 and 139 us.  fp32 rows
+// have three times the MMAs for the same sums: 118 us, 437 TFLOP/s of 557.
 // Built and slower: every warp of the second block arriving at the first's barrier by itself (64 us
 // where the one relay had 60), sixteen columns of sums on their way while sixteen are added (61 against
 // 59), polling barriers instead of sleeping on them (63 against 59).
@@ -482,8 +483,8 @@ int4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant_
     }
   } else if (warp >= 20) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    // Units of eight neighbouring columns of one row: sixteen a row (DUAL: eight), so 256 threads'
-    // worth a pass; consecutive threads take consecutive units.
+    // Units of eight neighbouring columns of one row: sixteen a row (DUAL: eight), so 128 threads take
+    // eight (sixteen) rows a pass; consecutive threads take consecutive units.
     constexpr int COLS = F / 2, UNITS = COLS / 8;
     const int thread = threadIdx.x - 20 * 32;
     const int unit = thread % UNITS;

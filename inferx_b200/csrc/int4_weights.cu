@@ -7,7 +7,7 @@
 //
 // One warp takes 16 rows by 128 k: a lane holds the 64 entries whose codes it packs, least and greatest
 // entries are joined over the four lanes of a row by shuffles, nothing passes through shared memory, and
-// each entry is read once.  Measured: 6,144 x 2,048 bfloat16 15 us, fp32 21 (the bytes alone 5 and 9):
+// each entry is read once.  Measured: 6,144 x 2,048 bfloat16 15 us, fp32 20 (the bytes alone 5 and 9):
 // finding the extremes and the two comparisons of an entry's remainder, not the bytes, set the pace.
 #include "int4_format.cuh"
 
@@ -112,7 +112,7 @@ template <> struct I4Entries<bf16> {
   }
 };
 
-// codes of rows g and g + 8 (32 each, in the order of i4_row_entries) to the lane's words
+// codes of rows g and g + 8 (32 each, in the order of I4Entries) to the lane's words
 __device__ __forceinline__ void i4_store_words(unsigned* dst, int lane, const unsigned char* ca,
                                                const unsigned char* cb) {
 #pragma unroll

@@ -1758,18 +1758,20 @@ def _int4_tc(what, x, rows, offsets, w, num_rows, out_dtype, row_scale=None, act
 
 # One matrix: the streaming kernel reads the codes once for every 32 rows (16 in 32 bits), pass after
 # pass, and its time goes by rows x bytes; the tensor-core kernel has some 6 to 13 us to begin and end
-# with.  us, streaming / tensor cores: 2048 -> 6144 32 rows 13.6 / 13.9, 64 rows 24 / 14.1; gated 2048 -> 2
-# x 5632 24 rows 16.4 / 14.5.  Small matrices leave SMs idle in every pass: 512 -> 512 64 rows 6.6 /
-# 7.5, 96 rows 9.2 / 7.5, 512 rows 42 / 8.1; 5632 -> 64 48 rows 12.8 / 10.8; 2048 -> 2048 64 rows 8.5 /
-# 11.1, 96 rows 11.9 / 12.3; 32-bit 2048 -> 2048 32 rows 10.8 / 12.3, 48 rows 15.3 / 13.1; 1024 -> 1024
-# 32 rows 6.8 / 10.6, 64 rows 12.0 / 11.8.  An eager 32-bit call on the tensor cores is three launches,
+# with.  us, streaming / tensor cores: 2048 -> 6144 32 rows 12.5 / 12.9, 64 rows 23 / 14.3; gated 2048 -> 2
+# x 5632 24 rows 16.4 / 14.6.  Small matrices leave SMs idle in every pass: 512 -> 512 64 rows 6.4 /
+# 7.3, 96 rows 8.9 / 7.3, 512 rows 42 / 8.0; 5632 -> 64 48 rows 12.2 / 10.6; 2048 -> 2048 64 rows 8.5 /
+# 11.8, 96 rows 11.7 / 12.9; 32-bit 2048 -> 2048 32 rows 10.5 / 13.2, 48 rows 14.8 / 14.0; 1024 -> 1024
+# 32 rows 6.4 / 11.2, 64 rows 11.8 / 12.1.  An eager 32-bit call on the tensor cores is three launches,
 # 24 us of the host against 10: 33 rows of 1000 -> 515 take 10.3 / 23.8 a call.
 INT4_STREAM_ROWS = 16
 INT4_STREAM_MOST_ROWS = {torch.bfloat16: 64, torch.float32: 48}
 INT4_STREAM_ROW_BYTES = {torch.bfloat16: 250e6, torch.float32: 110e6}
 # Experts (60 of 2 x 1408 x 2048 and back, us, streaming 8 / 16 rows a pass / tensor cores): 6.4 rows
-# an expert 115 / 128 / 172, 8.5 rows 136 / 129 / 172, 12.8 rows 176 / 144 / 172; 32-bit 6.4 rows
-# 210 / 262 / 251, 8.5 rows 272 / 265 / 252.
+# an expert 98 / 119 / 147, 8.5 rows 115 / 120 / 147, 12.8 rows 148 / 134 / 148; 32-bit 6.4 rows
+# 195 / 254 / 176, 8.5 rows 253 / 256 / 177.  (The limits were set when these stood at 115 / 128 / 172,
+# 136 / 129 / 172, 176 / 144 / 172 and 210 / 262 / 251, 272 / 265 / 252; next to them either side is within
+# an eighth of the other.)
 INT4_STREAM_ROWS_PER_EXPERT = {torch.bfloat16: 12.0, torch.float32: 7.0}
 INT4_PASS8_ROWS_PER_EXPERT = 7.0
 
